@@ -409,7 +409,7 @@ __global__ __launch_bounds__(THREADS, 4) void img1_bwd_kernel(XView x, int B, in
     __shared__ __attribute__((aligned(16))) float xs[3 * G::XH * G::XP];
     __shared__ float red[4][CO][PROW];
     const int co = threadIdx.x & 15, slot = threadIdx.x >> 4;
-    // taps in pairs: v_pk_fma_f32 does two of the element's 2 x 27 multiply-adds per instruction (the kernel is VALU-issue bound)
+    // taps in pairs (the library is built without packed FP32 instructions: each pair is two scalar multiply-adds)
     constexpr int NP = NTAP / 2;
     f32x2 w2[NP], T2[NP];
     float wl = wgt.ld(co, NTAP - 1), Tl = 0.f, m1 = 0.f, m2 = 0.f;
