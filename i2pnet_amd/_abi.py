@@ -115,6 +115,12 @@ DEVICE_ONLY = {
     "i2p_mask_fill": ["l", "i", "p", "p", "f", "p"],
     "i2p_pad_cols": ["i", "i", "i", "p", "p"],
     "i2p_strided_pick2": ["i"] * 7 + ["p"] * 4,
+    "i2p_rms_norm_fwd": ["l", "i", "i", "i", "p", "l", "p", "l", "p", "f", "p", "p", "p"],
+    "i2p_rms_norm_q8": ["l", "i", "i", "i", "p", "l", "p", "l", "p", "f", "i", "p", "p", "p"],
+    "i2p_rms_norm_bwd": ["l", "i", "i", "i", "p", "l", "p", "l", "p", "l", "p", "p", "p", "p", "p"],
+    "i2p_token_logprobs_fwd": ["l", "i", "i", "p", "l", "p", "l", "i"] + ["p"] * 6,
+    "i2p_token_logprobs_bwd": ["l", "i", "i", "p", "l", "p", "l"] + ["p"] * 5,
+    "i2p_clip_grad_norm": ["i", "p", "p", "p", "i", "i", "f", "p", "p", "p"],
 }
 # plain `int f(...)` helpers without a stream argument
 HELPERS = {
@@ -138,10 +144,14 @@ HELPERS = {
     "i2p_defer_compact_next": ["i", "i", "i"],
     "i2p_defer_pending": [],
     "i2p_defer_end": [],
+    "i2p_rms_norm_bwd_scratch": ["l", "i"],                         # returns long long (bytes)
+    "i2p_token_logprobs_scratch": ["l", "i", "i", "i"],             # returns long long (bytes)
+    "i2p_grad_norm_scratch": ["i", "p"],                            # returns long long (bytes)
     "i2p_ktime_enable": ["i"],
     "i2p_ktime_last_us": [],                                        # returns float (microseconds)
 }
-LONG_HELPERS = {"i2p_pair_lin_bwd_scratch", "i2p_pair_bias_bn_bwd_scratch", "i2p_gather_rows_grad_fx_scratch", "i2p_gemm_tn_scratch", "i2p_chain_sums_len", "i2p_chain_sync_words", "i2p_chain_bwd_slab"}
+LONG_HELPERS = {"i2p_pair_lin_bwd_scratch", "i2p_pair_bias_bn_bwd_scratch", "i2p_gather_rows_grad_fx_scratch", "i2p_gemm_tn_scratch", "i2p_chain_sums_len", "i2p_chain_sync_words", "i2p_chain_bwd_slab",
+                "i2p_rms_norm_bwd_scratch", "i2p_token_logprobs_scratch", "i2p_grad_norm_scratch"}
 
 FLOAT_HELPERS = {"i2p_ktime_last_us"}
 

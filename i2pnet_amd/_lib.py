@@ -18,7 +18,8 @@ class I2POpsError(RuntimeError):
     pass
 
 
-_ERRORS = {-1: "bad argument", -2: "kernel_size_H*kernel_size_W exceeds 150", -3: "K exceeds 150"}
+_ERRORS = {-1: "bad argument", -2: "kernel_size_H*kernel_size_W exceeds 150", -3: "K exceeds 150",
+           -4: "tensors of the list share memory"}
 
 
 def lib_path():

@@ -1,4 +1,6 @@
 """Learned-uncertainty pose loss (reference: compute_loss.py:102-133, `Get_loss`)."""
+from collections import namedtuple
+
 import torch
 
 from . import ops
@@ -53,3 +55,39 @@ def Get_loss(out3, out4, qq_gt, t_gt, w_x, w_q, cfg):
     per_level = loss_x * torch.exp(-w_x) + w_x + loss_q * torch.exp(-w_q) + w_q     # [2]  :121
     loss = 1.6 * per_level[0:1] + 0.8 * per_level[1:2]                               # shape [1] like the reference
     return loss, 1.6 * loss_q[0] + 0.8 * loss_q[1], 1.6 * loss_x[0] + 0.8 * loss_x[1]
+
+
+TokenLogprobs = namedtuple("TokenLogprobs", ["logp", "entropy", "top_logp", "top_ids"])
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, top, ignore_index):
+        logp, entropy, top_logp, top_ids, x2, ids, stat = ops.get_backend().token_logprobs_forward(logits, ids, top, ignore_index)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(top_logp, top_ids)
+        ctx.save_for_backward(x2, ids, stat, entropy)
+        ctx.ignore_index, ctx.shape = ignore_index, logits.shape
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, _g_top, _g_ids):
+        if g_logp is None and g_entropy is None:
+            return None, None, None, None
+        x2, ids, stat, entropy = ctx.saved_tensors
+        dx = ops.get_backend().token_logprobs_backward(x2, ids, ctx.ignore_index, stat, entropy, g_logp, g_entropy)
+        return dx.view(ctx.shape), None, None, None
+
+
+def token_logprobs(logits, ids, top=0, ignore_index=-100):
+    """Log probabilities of the candidates `ids` [...] under softmax(logits [..., v]), with the entropy of every row and its `top` best
+    alternatives -> TokenLogprobs(logp [...], entropy [...], top_logp [..., top], top_ids [..., top]), float32 and int64.  The matching loss of
+    points against pixels (or of any answer against its candidates) is -logp.mean(); entropy is the match's confidence.
+
+    logits: float32, bfloat16 or float16, any row pitch, up to 2^21 candidates; masked candidates are -inf or the type's lowest value.
+    ids: int64.  A row whose id is `ignore_index` is padding: it is not read, logp and entropy are 0, its alternatives -1 with -inf, its
+    gradient 0.  Any other id outside [0, v) makes that row's logp and gradient NaN (ids are not read on the host).  A row without
+    candidates (all -inf) has logp -inf, entropy 0 and gradient 0; a NaN or +inf makes the row's results NaN.
+    top: 0 .. min(v, 32); equal scores are listed by index.  logp and entropy are differentiable in logits, once; the alternatives are not."""
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, ids, int(top), int(ignore_index)))

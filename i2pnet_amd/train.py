@@ -140,6 +140,62 @@ class FlatAdam:
         self.lr_t.mul_(gamma)
 
 
+def _grad_list(parameters):
+    """the gradients meant by a list of parameters (those that have one) and plain gradient tensors"""
+    grads = []
+    for t in [parameters] if isinstance(parameters, torch.Tensor) else parameters:
+        if type(t) is torch.Tensor and not t.requires_grad:
+            grads.append(t)
+        elif not isinstance(t, torch.Tensor) or not t.is_leaf:
+            raise RuntimeError(f"parameters (leaves) or gradient tensors are wanted (got {type(t).__name__})")
+        elif t.grad is not None:
+            grads.append(t.grad)
+    return grads
+
+
+def _norm_kind(norm_type):
+    if float(norm_type) == 2.0:
+        return 0
+    if float(norm_type) == float("inf"):
+        return 1
+    raise ValueError(f"norm_type must be 2 or inf (got {norm_type})")
+
+
+@torch.no_grad()
+def grad_norm(parameters, norm_type=2.0):
+    """Global norm (2, or inf: the largest magnitude) of the gradients of `parameters` -> float32 0-d tensor on their device; the host does
+    not wait.  `parameters`: parameters, whose .grad is meant (those without one are skipped), or gradient tensors themselves."""
+    grads, kind = _grad_list(parameters), _norm_kind(norm_type)
+    if not grads:
+        return torch.zeros((), device="cuda")
+    return ops.get_backend().clip_grad_norm(grads, kind, None)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
+    """Clips the gradients of `parameters` to a global norm of at most `max_norm` (times min(1, max_norm / (norm + 1e-6))) and returns the norm
+    before it, without waiting for the device: what `FlatAdam.fused_clip_step` does for the trainer's flat buffer, for any list of
+    gradients (csrc/grad_norm.hip; reference: train20v2learn_wandb_proj.py:472-476).  In place, or into `out`, a flat float32 tensor that
+    gets the clipped gradients one behind the other (each in its storage's order) and leaves them as they are.
+
+    parameters: see `grad_norm`; dense float32, bfloat16 and float16 tensors of one device, mixed; tensors that share memory are refused
+    in place.  A NaN or inf norm makes every gradient NaN or 0, as torch's function does; error_if_nonfinite raises instead (it waits for
+    the device) and leaves them as they are."""
+    grads, kind, max_norm = _grad_list(parameters), _norm_kind(norm_type), float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    if not grads:
+        if out is not None and out.numel():
+            raise RuntimeError("out must be empty: there is no gradient")
+        return torch.zeros((), device="cuda")
+    be = ops.get_backend()
+    if error_if_nonfinite and not bool(torch.isfinite(be.clip_grad_norm(grads, kind, None))):
+        raise RuntimeError("the global norm of the gradients is not finite: they were not clipped")
+    total = be.clip_grad_norm(grads, kind, max_norm, out)
+    torch.autograd.graph.increment_version(grads if out is None else out)
+    return total
+
+
 # what a step reads of a loader sample dict (kitti_odometry_corr_lidarnone_proj.py:757-789 also carries strings
 # such as `path_info` and unused tensors such as `resize_img`: they never reach the device)
 STEP_KEYS = ("rgb", "lidar", "raw_point_xyz", "lidar_feats", "init_intrinsic", "init_extrinsic", "decalib_real_gt",

@@ -35,6 +35,12 @@ extern "C" {
 #define I2P_ERR_BAD_ARG   (-1)  /* negative size, NULL pointer with non-empty work          */
 #define I2P_ERR_WINDOW    (-2)  /* kernel_size_H*kernel_size_W > I2P_MAX_WINDOW               */
 #define I2P_ERR_K         (-3)  /* K > I2P_MAX_WINDOW                                         */
+#define I2P_ERR_OVERLAP   (-4)  /* tensors of one list share memory                           */
+
+/* storage types of the row operators (i2p_rms_norm_*, i2p_token_logprobs_*, i2p_clip_grad_norm) */
+#define I2P_F32  0
+#define I2P_BF16 1
+#define I2P_F16  2
 
 /* The reference keeps `int idx_w[150], idx_h[150]; float Dist[150]` per thread
  * (fused_conv_go.cu:52-53) and silently overflows beyond that; we reject instead. */
@@ -696,6 +702,48 @@ int i2p_strided_pick2(int B, int H, int W, int oh, int ow, int sh, int sw, const
 int i2p_kitti_points_build(int B, int sample_point, const void *table, const float *noise, float *lidar, float *raw, float *feats,
                            void *stream);
 int i2p_kitti_image_build(int B, int out_h, int out_w, const void *table, float *rgb, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Row operators of a training or matching step (not in the reference): any width, rows of pitch ld >= width (elements), storage types
+ * I2P_F32 / I2P_BF16 / I2P_F16, fp32 arithmetic, 1-byte alignment beyond the element's own not required.  Results are reproducible.
+ *
+ * Root-mean-square norm with the residual's addition: s [rows,d] = round(x + res) (res, s both NULL: the norm is of x itself),
+ * rstd f32 [rows] = 1/sqrt(mean(s^2) + eps) (NULL: not wanted), y [rows,d] = round(s * rstd * w); w [d] of type wdtype (I2P_F32 or
+ * dtype), NULL = ones.  s, y are dense.
+ * _q8: q u8 [rows,d] = OCP e4m3 bits of s * rstd * w / scale, scale f32 [rows, ceil(d / group)] = max |s * rstd * w| / 448 over the group's
+ * columns (1 where they are all zero); group a power of two, 32 .. 512, or 0 = the whole row.  A group with a NaN or inf has scale inf.
+ * _bwd: gy [rows,d], gs (gradient of s, NULL = none) -> dx [rows,d] (dense; the gradient of x and of res), dw [d] of type wdtype (NULL: not
+ * wanted); s, rstd as the forward left them; scratch: i2p_rms_norm_bwd_scratch(rows, d) bytes, needed with dw.
+ * --------------------------------------------------------------------------------------------- */
+int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr, const void *w,
+                     float eps, void *s, void *y, float *rstd, void *stream);
+int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr, const void *w,
+                    float eps, int group, void *s, unsigned char *q, float *scale, void *stream);
+long long i2p_rms_norm_bwd_scratch(long long rows, int d);
+int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, const void *s, long long lds, const void *gy, long long ldgy, const void *gs,
+                     long long ldgs, const void *w, const float *rstd, void *dx, void *dw, void *scratch, void *stream);
+/* Log probabilities of one given candidate per row of scores x [rows,v] (pitch ldx, v <= I2P_MAX_CANDIDATES), with the row's entropy and its `top` best alternatives
+ * (0 <= top <= min(v, I2P_MAX_TOP); equal scores in index order): logp, entropy f32 [rows], top_logp f32 / top_ids i64 [rows,top];
+ * stat f32 [rows,2] is for the backward.  ids i64 [rows]: a row with id == ignore is not read (logp = entropy = 0, top_logp = -inf,
+ * top_ids = -1, gradient 0); any other id outside [0, v) gives logp and gradient NaN.  A row of -inf: logp = -inf, entropy = 0, gradient 0;
+ * NaN or +inf in a row: NaN.  scratch: i2p_token_logprobs_scratch(rows, v, dtype, top) bytes.
+ * _bwd: g_logp, g_entropy f32 [rows] (either may be NULL = 0) -> dx [rows,v] (dense, of type dtype). */
+#define I2P_MAX_TOP 32
+#define I2P_MAX_CANDIDATES (1 << 21)
+long long i2p_token_logprobs_scratch(long long rows, int v, int dtype, int top);
+int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const void *x, long long ldx, const int64_t *ids, long long ignore, int top,
+                           float *logp, float *entropy, float *stat, float *top_logp, int64_t *top_ids, void *scratch, void *stream);
+int i2p_token_logprobs_bwd(long long rows, int v, int dtype, const void *x, long long ldx, const int64_t *ids, long long ignore,
+                           const float *stat, const float *entropy, const float *g_logp, const float *g_entropy, void *dx, void *stream);
+/* Global norm of n gradient tensors and clipping by it (what clip_grad_norm_ does to a list of parameters,
+ * train20v2learn_wandb_proj.py:472-476; i2p_clip_adam does it for the trainer's flat buffer).  grads / numel / dtype: HOST arrays of n
+ * device pointers, element counts and storage types (dense tensors, zero elements allowed); the kernels carry them by value, so the call
+ * may be captured.  kind 0: total f32 [1] = sqrt(sum g^2), 1: max |g|.  clip != 0: every gradient times min(1, max_norm / (total + 1e-6)),
+ * in place (out NULL; gradients within the limit are not written) or into the flat fp32 buffer `out`, tensor behind tensor.
+ * I2P_ERR_OVERLAP: tensors that would be written share memory.  scratch: i2p_grad_norm_scratch(n, numel) bytes. */
+long long i2p_grad_norm_scratch(int n, const long long *numel);
+int i2p_clip_grad_norm(int n, const void *const *grads, const long long *numel, const int *dtype, int kind, int clip, float max_norm,
+                       float *out, void *scratch, float *total, void *stream);
 
 /* Measurement hook (bench.py's roofline object): with i2p_ktime_enable(1) the launchers of wreg_bwd_fused_kernel (fp32) and
  * bwd_fused_bf16_kernel bracket the kernel alone with HIP events on the launch stream; i2p_ktime_last_us() waits for the last

@@ -1,0 +1,122 @@
+"""Row operators without a GPU: what is refused before any launch."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from i2pnet_amd import _lib, loss, modules, ops, train
+
+BAD, OVERLAP = "bad argument", "share memory"
+
+
+def call(name, *args):
+    _lib.call(name, *args)
+
+
+P = 4096        # stands for a device pointer: every call here is refused before anything is launched
+
+
+@pytest.mark.parametrize("change", [dict(rows=-1), dict(d=0), dict(d=-4), dict(dtype=3), dict(dtype=-1), dict(wdtype=2), dict(ldx=7), dict(ldr=7), dict(x=None),
+                                    dict(y=None), dict(s=None), dict(res=None)])
+def test_rms_norm_forward_refusals(change):
+    a = dict(rows=2, d=8, dtype=1, wdtype=0, x=P, ldx=8, res=P, ldr=8, w=P, eps=1e-6, s=P, y=P, rstd=P) | change
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_rms_norm_fwd", *a.values())
+
+
+@pytest.mark.parametrize("change", [dict(group=16), dict(group=48), dict(group=1024), dict(group=-32), dict(q=None), dict(scale=None), dict(d=0), dict(dtype=9),
+                                    dict(wdtype=1, dtype=2)])
+def test_rms_norm_q8_refusals(change):
+    a = dict(rows=2, d=8, dtype=1, wdtype=0, x=P, ldx=8, res=None, ldr=0, w=P, eps=1e-6, group=32, s=None, q=P, scale=P) | change
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_rms_norm_q8", *a.values())
+
+
+@pytest.mark.parametrize("change", [dict(rows=0), dict(d=0), dict(dtype=3), dict(lds=3), dict(ldgy=3), dict(ldgs=3), dict(s=None), dict(gy=None), dict(rstd=None),
+                                    dict(dx=None), dict(scratch=None)])
+def test_rms_norm_backward_refusals(change):
+    a = dict(rows=2, d=8, dtype=1, wdtype=0, s=P, lds=8, gy=P, ldgy=8, gs=P, ldgs=8, w=P, rstd=P, dx=P, dw=P, scratch=P) | change
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_rms_norm_bwd", *a.values())
+
+
+@pytest.mark.parametrize("change", [dict(rows=-1), dict(v=0), dict(v=(1 << 21) + 1, ldx=1 << 22), dict(dtype=3), dict(ldx=3), dict(top=-1), dict(top=9), dict(v=100, ldx=100, top=33),
+                                    dict(x=None), dict(ids=None), dict(logp=None), dict(entropy=None), dict(stat=None), dict(top_logp=None), dict(top_ids=None)])
+def test_token_logprobs_refusals(change):
+    a = dict(rows=2, v=8, dtype=1, x=P, ldx=8, ids=P, ignore=-100, top=2, logp=P, entropy=P, stat=P, top_logp=P, top_ids=P, scratch=P) | change
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_token_logprobs_fwd", *a.values())
+
+
+@pytest.mark.parametrize("change", [dict(v=0), dict(dtype=3), dict(ldx=3), dict(x=None), dict(ids=None), dict(stat=None), dict(entropy=None), dict(dx=None)])
+def test_token_logprobs_backward_refusals(change):
+    a = dict(rows=2, v=8, dtype=1, x=P, ldx=8, ids=P, ignore=-100, stat=P, entropy=P, gl=None, gh=None, dx=P) | change
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_token_logprobs_bwd", *a.values())
+
+
+def clip(ptrs, sizes, dtypes, kind=0, do=1, limit=1.0, out=None, scratch=P, total=P, n=None):
+    a = (C.c_void_p * max(1, len(ptrs)))(*ptrs)
+    b = (C.c_longlong * max(1, len(sizes)))(*sizes)
+    c = (C.c_int * max(1, len(dtypes)))(*dtypes)
+    call("i2p_clip_grad_norm", len(ptrs) if n is None else n, C.cast(a, C.c_void_p), C.cast(b, C.c_void_p), C.cast(c, C.c_void_p), kind, do, limit, out, scratch, total)
+
+
+@pytest.mark.parametrize("args,what", [
+    (([P], [-1], [0]), BAD), (([P], [4], [3]), BAD), (([None], [4], [0]), BAD), (([P + 2], [4], [0]), BAD), (([P + 1], [4], [1]), BAD), (([1 << 50], [4], [0]), BAD),
+    (([P, P], [1 << 44, 1], [0, 0]), BAD),
+    (([P, P], [4, 4], [0, 0]), OVERLAP), (([P, P + 12], [4, 4], [0, 0]), OVERLAP), (([P + 14, P], [4, 8], [1, 1]), OVERLAP)])
+def test_clip_grad_norm_refusals(args, what):
+    with pytest.raises(_lib.I2POpsError, match=what):
+        clip(*args)
+
+
+@pytest.mark.parametrize("change", [dict(kind=2), dict(kind=-1), dict(limit=-1.0), dict(limit=math.nan), dict(scratch=None), dict(total=None), dict(n=-1)])
+def test_clip_grad_norm_argument_refusals(change):
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        clip([P], [4], [0], **change)
+
+
+def test_clip_grad_norm_output_must_not_overlap():
+    for out in (P, P + 12, P - 28):
+        with pytest.raises(_lib.I2POpsError, match=OVERLAP):
+            clip([P, P + 1024], [4, 4], [0, 0], out=out)
+
+
+def test_scratch_sizes():
+    n = (C.c_longlong * 3)(1, 0, (1 << 31) + 5)
+    assert _lib.helper("i2p_grad_norm_scratch", 3, C.cast(n, C.c_void_p)) >= 8
+    assert _lib.helper("i2p_grad_norm_scratch", 0, None) >= 8
+    assert _lib.helper("i2p_rms_norm_bwd_scratch", 0, 8) == 0 and _lib.helper("i2p_rms_norm_bwd_scratch", 1000000, 4096) >= 4096 * 4
+
+
+def test_host_tensors_and_types_are_refused():
+    x, w = torch.zeros(2, 8), torch.ones(8)
+    for f in (lambda: modules.rms_norm(x, w), lambda: modules.rms_norm_q8(x, w), lambda: loss.token_logprobs(x, torch.zeros(2, dtype=torch.long)),
+              lambda: train.clip_grad_norm_([x], 1.0), lambda: train.grad_norm([x])):
+        with pytest.raises(RuntimeError, match="cuda"):
+            f()
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        train.clip_grad_norm_([x.double()], 1.0)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        modules.rms_norm_q8(x.clone().requires_grad_(True), w)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            train.clip_grad_norm_([x], bad)
+    with pytest.raises(ValueError, match="norm_type"):
+        train.clip_grad_norm_([x], 1.0, norm_type=1)
+    with pytest.raises(RuntimeError, match="leaves"):
+        train.clip_grad_norm_([(x.clone().requires_grad_(True) * 2)], 1.0)
+    with pytest.raises(RuntimeError, match="leaves"):
+        train.clip_grad_norm_([3.0], 1.0)
+
+
+def test_lists_of_parameters():
+    a, b, c = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    a.grad = torch.ones(3)
+    c.requires_grad_(False)
+    raw = torch.zeros(2)
+    assert train._grad_list([a, b, c, raw])[0] is a.grad and len(train._grad_list([a, b, c, raw])) == 2
+    assert train._grad_list(raw)[0] is raw and train._grad_list(x for x in ()) == []
+    assert isinstance(ops.MAX_TOP, int)
