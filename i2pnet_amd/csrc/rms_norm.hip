@@ -2,106 +2,364 @@
 //
 //   s = round(x + res)             the residual stream, kept in the inputs' type: the norm is of the stream as it is stored
 //   rstd = 1 / sqrt(mean(s^2) + eps),  y = round(s * rstd * w)
-//   8 bits: scale = max |s rstd w| / 448 over a group of columns (1 where the group is all zero), q = e4m3(s rstd w / scale)
+//   8 bits: scale = max |s rstd w| / 448 over a group of columns (1 where that is below the smallest normal number), q = e4m3(s rstd w / scale)
 //   backward, t = gy * w, xh = s * rstd:  dx = dres = round(rstd * (t - xh * mean(t * xh)) + gs),  dw = sum over rows of gy * xh
 //
-// Sums are fp32.  dw is summed per block over the rows it owns and then over the blocks in index order: reproducible.
+// All of it is bound by memory: a row lives in the registers of the TPR threads that share it (NV 16-byte vectors each, the 16-bit types
+// packed), so every input is read once and every output written once.  Short rows are shared by 16 lanes or one wave (no barrier, several
+// rows per block), longer ones by a block of 256 or 1024.  Sums are fp32; dw is summed per block over the rows it owns (fp32 registers),
+// then over the blocks in index order: reproducible.
 #include "rows_common.h"
 
 namespace {
 
-constexpr int T = 256;
+constexpr int DW_COLS = 32, DW_LANES = 32;      // dw reduction: columns and row lanes of a block
 
-template <int DT, int WT, bool Q8>
-__global__ __launch_bounds__(T) void rms_fwd_kernel(long long rows, int d, const void *__restrict__ x, long long ldx, const void *__restrict__ res,
-                                                    long long ldr, const void *__restrict__ w, float eps, void *__restrict__ s,
-                                                    void *__restrict__ y, float *__restrict__ rstd_out, int group, unsigned char *__restrict__ q,
-                                                    float *__restrict__ scale) {
-    __shared__ float red[T / 64];
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        float acc = 0.f;
-        auto at = [&](int i) {
-            float v = ld1<DT>(x, row * ldx + i);
-            if (res) v = round1<DT>(v + ld1<DT>(res, row * ldr + i));
-            return v;
-        };
-        for (int i = threadIdx.x; i < d; i += T) {
-            const float v = at(i);
-            if (s) st1<DT>(s, row * d + i, v);
-            acc += v * v;
+// sum (or maximum of non-negative values' bits) over the TPR threads of a row; every one gets it.  A block-wide row uses red[waves]; calls
+// alternate between two such arrays, so that one barrier each is enough
+template <int TPR, class V, class Op> __device__ __forceinline__ V row_reduce(V v, V *red, Op op) {
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v = op(v, (V)__shfl_xor(v, o, 64));
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) v = op(v, red[w]);
+    }
+    return v;
+}
+struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+struct Max { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; } };
+
+// the weights of a vector of columns (ones where there is no weight)
+template <int DT, bool TINY> __device__ __forceinline__ void ld_weight(const void *w, int wdtype, const Col<DT, TINY> &c, int d, float (&f)[i2p_vec(DT)]) {
+    constexpr int VE = i2p_vec(DT);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = 1.f;
+    if (!w || !c.in) return;
+    if (wdtype == DT) unpack<DT>(c.load((const char *)w, d), f);
+    else if (!TINY) {                            // fp32 weights of a 16-bit row: two vectors
+        float4 a[2];
+        __builtin_memcpy(a, (const float *)w + c.at, 4 * VE);
+        f[0] = a[0].x; f[1] = a[0].y; f[2] = a[0].z; f[3] = a[0].w;
+        if constexpr (VE == 8) { f[4] = a[1].x; f[5] = a[1].y; f[6] = a[1].z; f[7] = a[1].w; }
+    } else
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+            if (c.at + e < d) f[e] = ((const float *)w)[c.at + e];
+}
+
+struct FwdArgs {
+    long long rows; int d, wdtype; const char *x; long long ldx; const char *res; long long ldr; const void *w; float eps; char *s, *y;
+    float *rstd; int group; unsigned char *q; float *scale;
+};
+
+__device__ __forceinline__ float scale_of(unsigned bits) {
+    if (bits > 0x7f7fffffu) return __builtin_inff();
+    const float sc = __uint_as_float(bits) / 448.f;
+    return sc < 1.17549435e-38f ? 1.f : sc;
+}
+
+template <int DT, int TPR, int NV, bool Q8>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(FwdArgs a) {
+    constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT), BLOCK = TPR < 256 ? 256 : TPR;
+    constexpr bool TINY = TPR == 16;
+    __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+    __shared__ unsigned mred[TPR > 64 ? TPR / 64 : 1];
+    const long long row = (long long)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+    if (TPR < BLOCK && row >= a.rows) return;                   // (a block-wide row always exists)
+    const int t = threadIdx.x % TPR, d = a.d;
+    auto col = [&](int j) { return Col<DT, TINY>(j * TPR + t, d); };
+    const char *x = a.x + row * a.ldx * ES;
+    uint4 v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = col(j).load(x, d);
+    if (a.res) {
+        const char *r = a.res + row * a.ldr * ES;
+        uint4 u[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) u[j] = col(j).load(r, d);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float f[VE], g[VE];
+            unpack<DT>(v[j], f); unpack<DT>(u[j], g);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[e] += g[e];
+            v[j] = pack<DT>(f);
+            col(j).store(a.s + row * d * ES, d, v[j]);
         }
-        const float rstd = 1.f / sqrtf(block_reduce<false>(acc, red) / (float)d + eps);
-        auto val = [&](int i) { return at(i) * rstd * (w ? ld1<WT>(w, i) : 1.f); };
-        if constexpr (!Q8) {
-            if (rstd_out && threadIdx.x == 0) rstd_out[row] = rstd;
-            for (int i = threadIdx.x; i < d; i += T) st1<DT>(y, row * d + i, val(i));
-        } else {
-            const int width = group ? group : d, ng = (d + width - 1) / width;
-            for (int g = 0; g < ng; ++g) {
-                const int hi = min(d, (g + 1) * width);
-                float m = 0.f;
-                bool nan = false;
-                for (int i = g * width + threadIdx.x; i < hi; i += T) { const float v = fabsf(val(i)); m = fmaxf(m, v); nan |= v != v; }
-                m = block_reduce<true>(nan ? __builtin_inff() : m, red);
-                float sc = m / 448.f;
-                if (!(sc > 0.f)) sc = 1.f;
-                if (threadIdx.x == 0) scale[row * ng + g] = sc;
-                for (int i = g * width + threadIdx.x; i < hi; i += T) q[row * d + i] = (unsigned char)e4m3_pack4(val(i) / sc, 0.f, 0.f, 0.f);
+    }
+    float acc = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float f[VE];
+        unpack<DT>(v[j], f);
+        const Col<DT, TINY> c = col(j);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) acc += e >= c.skip ? f[e] * f[e] : 0.f;        // (what is past the row was read as 0)
+    }
+    const float rstd = 1.f / sqrtf(row_reduce<TPR>(acc, red, Add{}) / (float)d + a.eps);
+    if constexpr (!Q8) {
+        if (a.rstd && t == 0) a.rstd[row] = rstd;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float f[VE], w[VE];
+            unpack<DT>(v[j], f);
+            ld_weight<DT>(a.w, a.wdtype, col(j), d, w);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[e] = f[e] * rstd * w[e];
+            col(j).store(a.y + row * d * ES, d, pack<DT>(f));
+        }
+    } else {
+        unsigned char *q = a.q + row * d;
+        unsigned m[NV], all = 0u;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const Col<DT, TINY> c = col(j);
+            float f[VE], w[VE];
+            unpack<DT>(v[j], f);
+            ld_weight<DT>(a.w, a.wdtype, c, d, w);
+            m[j] = 0u;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) { const unsigned b = __float_as_uint(f[e] * rstd * w[e]) & 0x7fffffffu; if (c.counts(e, d) && b > m[j]) m[j] = b; }
+            all = m[j] > all ? m[j] : all;
+        }
+        // a group of columns is a run of group / VE lanes of one vector number (all TPR of a short row)
+        const int lanes = a.group ? min(a.group / VE, TPR) : 0, ng = a.group ? (d + a.group - 1) / a.group : 1;
+        if (!a.group) all = row_reduce<TPR>(all, mred, Max{});
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const Col<DT, TINY> c = col(j);
+            unsigned b = all;
+            if (a.group) {
+                b = m[j];
+                for (int o = lanes >> 1; o > 0; o >>= 1) { const unsigned u = (unsigned)__shfl_xor((int)b, o, 64); b = u > b ? u : b; }
+            }
+            if (!c.in) continue;
+            const float sc = scale_of(b), inv = 1.f / sc;
+            if (a.group ? (t & (lanes - 1)) == 0 : (t | j) == 0) a.scale[row * ng + (a.group ? (j * TPR + t) * VE / a.group : 0)] = sc;
+            float f[VE], w[VE];
+            unpack<DT>(v[j], f);
+            ld_weight<DT>(a.w, a.wdtype, c, d, w);
+            unsigned u[VE / 4];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[e] = f[e] * rstd * w[e] * inv;
+#pragma unroll
+            for (int k = 0; k < VE / 4; ++k) u[k] = e4m3_pack4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            if (!c.skip && c.at + VE <= d) __builtin_memcpy(q + c.at, u, VE);
+            else {                               // (the elements before may belong to another group)
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    if (c.counts(e, d)) q[c.at + e] = (unsigned char)(u[e >> 2] >> (8 * (e & 3)));
             }
         }
     }
 }
 
-template <int DT, int WT>
-__global__ __launch_bounds__(T) void rms_bwd_kernel(long long rows, int d, const void *__restrict__ s, long long lds, const void *__restrict__ gy,
-                                                    long long ldg, const void *__restrict__ gs, long long ldgs, const void *__restrict__ w,
-                                                    const float *__restrict__ rstd_in, void *__restrict__ dx, float *__restrict__ part) {
-    __shared__ float red[T / 64];
-    float *my = part ? part + (long long)blockIdx.x * d : nullptr;
-    if (my)
-        for (int i = threadIdx.x; i < d; i += T) my[i] = 0.f;
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        const float rstd = rstd_in[row];
-        float acc = 0.f;
-        for (int i = threadIdx.x; i < d; i += T) {
-            const float xh = ld1<DT>(s, row * lds + i) * rstd, g = ld1<DT>(gy, row * ldg + i);
-            acc += g * (w ? ld1<WT>(w, i) : 1.f) * xh;
-            if (my) my[i] += g * xh;
+struct BwdArgs {
+    long long rows; int d, wdtype; const char *s; long long lds; const char *gy; long long ldg; const char *gs; long long ldgs; const void *w;
+    const float *rstd; char *dx; float *part;
+};
+
+// Every group of TPR threads walks rows in steps of the grid
+template <int DT, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(BwdArgs a) {
+    constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
+    constexpr bool TINY = TPR == 16;
+    __shared__ float red[2][TPR > 64 ? TPR / 64 : 1];
+    __shared__ float cols[RPB > 1 ? BLOCK * VE : 1];
+    const int t = threadIdx.x % TPR, d = a.d;
+    auto col = [&](int j) { return Col<DT, TINY>(j * TPR + t, d); };
+    const long long step = (long long)gridDim.x * RPB;
+    float dw[NV][VE] = {};
+    int flip = 0;
+    for (long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR; row < a.rows; row += step, flip ^= 1) {
+        uint4 xs[NV], gg[NV], ex[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            xs[j] = col(j).load(a.s + row * a.lds * ES, d);
+            gg[j] = col(j).load(a.gy + row * a.ldg * ES, d);
+            if (a.gs) ex[j] = col(j).load(a.gs + row * a.ldgs * ES, d);
         }
-        const float mean = block_reduce<false>(acc, red) / (float)d;
-        for (int i = threadIdx.x; i < d; i += T) {
-            const float xh = ld1<DT>(s, row * lds + i) * rstd, t = ld1<DT>(gy, row * ldg + i) * (w ? ld1<WT>(w, i) : 1.f);
-            float v = rstd * (t - xh * mean);
-            if (gs) v += ld1<DT>(gs, row * ldgs + i);
-            st1<DT>(dx, row * d + i, v);
+        const float rstd = a.rstd[row];
+        float acc = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const Col<DT, TINY> c = col(j);
+            float f[VE], g[VE], w[VE];
+            unpack<DT>(xs[j], f); unpack<DT>(gg[j], g);
+            ld_weight<DT>(a.w, a.wdtype, c, d, w);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) { const float p = g[e] * (f[e] * rstd); dw[j][e] += p; acc += e >= c.skip ? p * w[e] : 0.f; }
+        }
+        const float mean = row_reduce<TPR>(acc, red[flip], Add{}) / (float)d;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float f[VE], g[VE], w[VE], h[VE] = {};
+            unpack<DT>(xs[j], f); unpack<DT>(gg[j], g);
+            if (a.gs) unpack<DT>(ex[j], h);
+            ld_weight<DT>(a.w, a.wdtype, col(j), d, w);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[e] = rstd * (g[e] * w[e] - f[e] * rstd * mean) + h[e];
+            col(j).store(a.dx + row * d * ES, d, pack<DT>(f));
+        }
+    }
+    if (!a.part) return;
+    float *out = a.part + (long long)blockIdx.x * d;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        if constexpr (RPB > 1) {                 // the block's groups, summed in order
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VE; ++e) cols[threadIdx.x * VE + e] = dw[j][e];
+            __syncthreads();
+            if (threadIdx.x < TPR) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    float v = 0.f;
+                    for (int g = 0; g < RPB; ++g) v += cols[(g * TPR + t) * VE + e];
+                    dw[j][e] = v;
+                }
+            }
+        }
+        if (RPB == 1 || threadIdx.x < TPR) {
+            const Col<DT, TINY> c = col(j);
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (c.counts(e, d)) out[c.at + e] = dw[j][e];
         }
     }
 }
 
-template <int WT> __global__ __launch_bounds__(T) void rms_dw_kernel(int nblk, int d, const float *__restrict__ part, void *__restrict__ dw) {
-    const int i = blockIdx.x * T + threadIdx.x;
-    if (i >= d) return;
-    float t = 0.f;
-    for (int b = 0; b < nblk; ++b) t += part[(long long)b * d + i];
-    st1<WT>(dw, i, t);
+__global__ __launch_bounds__(DW_COLS * DW_LANES) void rms_dw_kernel(int nblk, int d, const float *__restrict__ part, void *__restrict__ dw, int wdtype) {
+    __shared__ float sum[DW_LANES][DW_COLS + 1];
+    const int c = threadIdx.x % DW_COLS, l = threadIdx.x / DW_COLS, i = blockIdx.x * DW_COLS + c;
+    float v = 0.f;
+    if (i < d)
+#pragma unroll 4
+        for (int b = l; b < nblk; b += DW_LANES) v += part[(long long)b * d + i];
+    sum[l][c] = v;
+    __syncthreads();
+    if (l || i >= d) return;
+    for (int k = 1; k < DW_LANES; ++k) v += sum[k][c];
+    if (wdtype == I2P_F32) st1<I2P_F32>(dw, i, v);
+    else if (wdtype == I2P_BF16) st1<I2P_BF16>(dw, i, v);
+    else st1<I2P_F16>(dw, i, v);
 }
 
-inline long long bwd_blocks(long long rows) { return rows < 512 ? rows : 512; }
+// ---- rows longer than the registers of a block: 1024 threads walk them, reading twice --------------------------------------------------
+constexpr int LT = 1024;
+
+__device__ __forceinline__ float weight1(const void *w, int wdtype, int i) {
+    return !w ? 1.f : wdtype == I2P_F32 ? ld1<I2P_F32>(w, i) : wdtype == I2P_BF16 ? ld1<I2P_BF16>(w, i) : ld1<I2P_F16>(w, i);
+}
+
+template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_kernel(FwdArgs a) {
+    constexpr int ES = i2p_esize(DT);
+    __shared__ float red[LT / 64];
+    const int d = a.d;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const char *x = a.x + row * a.ldx * ES, *r = a.res + row * a.ldr * ES;
+        auto at = [&](int i) {
+            float v = ld1<DT>(x, i);
+            if (a.res) v = round1<DT>(v + ld1<DT>(r, i));
+            return v;
+        };
+        float acc = 0.f;
+        for (int i = threadIdx.x; i < d; i += LT) {
+            const float v = at(i);
+            if (a.s) st1<DT>(a.s, row * d + i, v);
+            acc += v * v;
+        }
+        const float rstd = 1.f / sqrtf(block_reduce<false>(acc, red) / (float)d + a.eps);
+        auto val = [&](int i) { return at(i) * rstd * weight1(a.w, a.wdtype, i); };
+        if constexpr (!Q8) {
+            if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+            for (int i = threadIdx.x; i < d; i += LT) st1<DT>(a.y, row * d + i, val(i));
+        } else if (a.group) {                    // a wave per group
+            const int ng = (d + a.group - 1) / a.group, lane = threadIdx.x & 63;
+            for (int g = threadIdx.x >> 6; g < ng; g += LT / 64) {
+                const int hi = min(d, (g + 1) * a.group);
+                unsigned m = 0u;
+                for (int i = g * a.group + lane; i < hi; i += 64) { const unsigned b = __float_as_uint(val(i)) & 0x7fffffffu; m = b > m ? b : m; }
+                m = row_reduce<64>(m, (unsigned *)nullptr, Max{});
+                const float sc = scale_of(m), inv = 1.f / sc;
+                if (lane == 0) a.scale[row * ng + g] = sc;
+                for (int i = g * a.group + lane; i < hi; i += 64) a.q[row * d + i] = (unsigned char)e4m3_pack4(val(i) * inv, 0.f, 0.f, 0.f);
+            }
+        } else {
+            unsigned m = 0u;
+            for (int i = threadIdx.x; i < d; i += LT) { const unsigned b = __float_as_uint(val(i)) & 0x7fffffffu; m = b > m ? b : m; }
+            __syncthreads();
+            m = row_reduce<LT>(m, (unsigned *)red, Max{});
+            const float sc = scale_of(m), inv = 1.f / sc;
+            if (threadIdx.x == 0) a.scale[row] = sc;
+            for (int i = threadIdx.x; i < d; i += LT) a.q[row * d + i] = (unsigned char)e4m3_pack4(val(i) * inv, 0.f, 0.f, 0.f);
+            __syncthreads();
+        }
+    }
+}
+
+template <int DT> __global__ __launch_bounds__(LT) void rms_bwd_long_kernel(BwdArgs a) {
+    constexpr int ES = i2p_esize(DT);
+    __shared__ float red[LT / 64];
+    const int d = a.d;
+    float *my = a.part ? a.part + (long long)blockIdx.x * d : nullptr;
+    if (my)
+        for (int i = threadIdx.x; i < d; i += LT) my[i] = 0.f;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const char *s = a.s + row * a.lds * ES, *gy = a.gy + row * a.ldg * ES, *gs = a.gs + row * a.ldgs * ES;
+        const float rstd = a.rstd[row];
+        float acc = 0.f;
+        for (int i = threadIdx.x; i < d; i += LT) {
+            const float c = ld1<DT>(gy, i) * (ld1<DT>(s, i) * rstd);
+            acc += c * weight1(a.w, a.wdtype, i);
+            if (my) my[i] += c;
+        }
+        const float mean = block_reduce<false>(acc, red) / (float)d;
+        for (int i = threadIdx.x; i < d; i += LT) {
+            float v = rstd * (ld1<DT>(gy, i) * weight1(a.w, a.wdtype, i) - ld1<DT>(s, i) * rstd * mean);
+            if (a.gs) v += ld1<DT>(gs, i);
+            st1<DT>(a.dx, row * d + i, v);
+        }
+    }
+}
+
 inline bool types_ok(int dtype, int wdtype) {
     return dtype >= I2P_F32 && dtype <= I2P_F16 && (wdtype == I2P_F32 || wdtype == dtype);
 }
 
-// calls f(DT, WT) as integral constants
-template <class F> void by_type(int dtype, int wdtype, F f) {
+constexpr long long BWD_BLOCKS = 512;
+inline long long bwd_blocks(long long rows) { return rows < BWD_BLOCKS ? rows : BWD_BLOCKS; }
+
+// f(DT, TPR, NV) for rows of d elements; false: the row does not fit the registers of a block
+template <int DT, class F> bool by_width(int d, F f) {
     using std::integral_constant;
-    if (dtype == I2P_F32) f(integral_constant<int, I2P_F32>{}, integral_constant<int, I2P_F32>{});
-    else if (dtype == I2P_BF16) {
-        if (wdtype == I2P_F32) f(integral_constant<int, I2P_BF16>{}, integral_constant<int, I2P_F32>{});
-        else f(integral_constant<int, I2P_BF16>{}, integral_constant<int, I2P_BF16>{});
-    } else {
-        if (wdtype == I2P_F32) f(integral_constant<int, I2P_F16>{}, integral_constant<int, I2P_F32>{});
-        else f(integral_constant<int, I2P_F16>{}, integral_constant<int, I2P_F16>{});
-    }
+    const long long n = ((long long)d + i2p_vec(DT) - 1) / i2p_vec(DT);
+#define I2P_ROW(TPR, NV) if (n <= (TPR) * (NV)) { f(integral_constant<int, DT>{}, integral_constant<int, TPR>{}, integral_constant<int, NV>{}); return true; }
+    I2P_ROW(16, 1) I2P_ROW(64, 1) I2P_ROW(64, 2) I2P_ROW(256, 1) I2P_ROW(256, 2) I2P_ROW(256, 4) I2P_ROW(1024, 2) I2P_ROW(1024, 4)
+#undef I2P_ROW
+    return false;
+}
+template <class F, class G> void by_row(int dtype, int d, F f, G longer, int group = 0) {
+    // (512 columns of fp32 are two waves' vectors: such groups take the long-row kernel unless they cover the row)
+    if (dtype == I2P_F32) { if ((group > 256 && d > 256) || !by_width<I2P_F32>(d, f)) longer(std::integral_constant<int, I2P_F32>{}); }
+    else if (dtype == I2P_BF16) { if (!by_width<I2P_BF16>(d, f)) longer(std::integral_constant<int, I2P_BF16>{}); }
+    else if (!by_width<I2P_F16>(d, f)) longer(std::integral_constant<int, I2P_F16>{});
+}
+
+template <bool Q8> int launch_fwd(int dtype, const FwdArgs &a, void *stream) {
+    if ((a.rows + 3) / 4 > 0x7fffffffll) return I2P_ERR_BAD_ARG;
+    by_row(dtype, a.d, [&](auto dt, auto tpr, auto nv) {
+        constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
+        hipLaunchKernelGGL((rms_fwd_kernel<dt.value, tpr.value, nv.value, Q8>), dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(BLOCK), 0,
+                           (hipStream_t)stream, a);
+    }, [&](auto dt) {
+        hipLaunchKernelGGL((rms_fwd_long_kernel<dt.value, Q8>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), dim3(LT), 0,
+                           (hipStream_t)stream, a);
+    }, a.group);
+    I2P_RETURN_LAUNCH_STATUS();
 }
 
 }  // namespace
@@ -110,13 +368,9 @@ extern "C" int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, co
                                 const void *w, float eps, void *s, void *y, float *rstd, void *stream) {
     if (rows < 0 || d <= 0 || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
-    if (!x || !y) return I2P_ERR_BAD_ARG;
-    const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : (1 << 20));
-    by_type(dtype, wdtype, [&](auto dt, auto wt) {
-        hipLaunchKernelGGL((rms_fwd_kernel<dt.value, wt.value, false>), dim3(grid), dim3(T), 0, (hipStream_t)stream, rows, d, x, ldx, res, ldr, w,
-                           eps, s, y, rstd, 0, (unsigned char *)nullptr, (float *)nullptr);
-    });
-    I2P_RETURN_LAUNCH_STATUS();
+    if (!x || !y || rows > 0x7fffffffll) return I2P_ERR_BAD_ARG;
+    return launch_fwd<false>(dtype, FwdArgs{rows, d, wdtype, (const char *)x, ldx, (const char *)res, ldr, w, eps, (char *)s, (char *)y, rstd, 0,
+                                            nullptr, nullptr}, stream);
 }
 
 extern "C" int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr,
@@ -124,13 +378,9 @@ extern "C" int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, con
     if (rows < 0 || d <= 0 || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
     if (group != 0 && (group < 32 || group > 512 || (group & (group - 1)))) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
-    if (!x || !q || !scale) return I2P_ERR_BAD_ARG;
-    const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : (1 << 20));
-    by_type(dtype, wdtype, [&](auto dt, auto wt) {
-        hipLaunchKernelGGL((rms_fwd_kernel<dt.value, wt.value, true>), dim3(grid), dim3(T), 0, (hipStream_t)stream, rows, d, x, ldx, res, ldr, w,
-                           eps, s, (void *)nullptr, (float *)nullptr, group, q, scale);
-    });
-    I2P_RETURN_LAUNCH_STATUS();
+    if (!x || !q || !scale || rows > 0x7fffffffll) return I2P_ERR_BAD_ARG;
+    return launch_fwd<true>(dtype, FwdArgs{rows, d, wdtype, (const char *)x, ldx, (const char *)res, ldr, w, eps, (char *)s, nullptr, nullptr, group,
+                                           q, scale}, stream);
 }
 
 extern "C" long long i2p_rms_norm_bwd_scratch(long long rows, int d) { return rows <= 0 || d <= 0 ? 0 : bwd_blocks(rows) * d * 4; }
@@ -139,13 +389,19 @@ extern "C" int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, co
                                 const void *gs, long long ldgs, const void *w, const float *rstd, void *dx, void *dw, void *scratch, void *stream) {
     if (rows <= 0 || d <= 0 || !types_ok(dtype, wdtype) || lds < d || ldgy < d || (gs && ldgs < d)) return I2P_ERR_BAD_ARG;
     if (!s || !gy || !rstd || !dx || (dw && !scratch)) return I2P_ERR_BAD_ARG;
-    const int nblk = (int)bwd_blocks(rows);
-    float *part = dw ? (float *)scratch : nullptr;
-    by_type(dtype, wdtype, [&](auto dt, auto wt) {
-        hipLaunchKernelGGL((rms_bwd_kernel<dt.value, wt.value>), dim3(nblk), dim3(T), 0, (hipStream_t)stream, rows, d, s, lds, gy, ldgy, gs, ldgs,
-                           w, rstd, dx, part);
-        if (dw)
-            hipLaunchKernelGGL((rms_dw_kernel<wt.value>), dim3((d + T - 1) / T), dim3(T), 0, (hipStream_t)stream, nblk, d, part, dw);
+    const BwdArgs a{rows, d, wdtype, (const char *)s, lds, (const char *)gy, ldgy, (const char *)gs, ldgs, w, rstd, (char *)dx,
+                    dw ? (float *)scratch : nullptr};
+    long long nblk = 0;
+    by_row(dtype, d, [&](auto dt, auto tpr, auto nv) {
+        constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
+        nblk = bwd_blocks((rows + RPB - 1) / RPB);
+        hipLaunchKernelGGL((rms_bwd_kernel<dt.value, tpr.value, nv.value>), dim3((unsigned)nblk), dim3(BLOCK), 0, (hipStream_t)stream, a);
+    }, [&](auto dt) {
+        nblk = bwd_blocks(rows);
+        hipLaunchKernelGGL((rms_bwd_long_kernel<dt.value>), dim3((unsigned)nblk), dim3(LT), 0, (hipStream_t)stream, a);
     });
+    if (dw)
+        hipLaunchKernelGGL(rms_dw_kernel, dim3((unsigned)((d + DW_COLS - 1) / DW_COLS)), dim3(DW_COLS * DW_LANES), 0, (hipStream_t)stream, (int)nblk, d,
+                           a.part, dw, wdtype);
     I2P_RETURN_LAUNCH_STATUS();
 }

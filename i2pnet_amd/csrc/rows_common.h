@@ -1,8 +1,13 @@
 // Storage types of the row operators (rms_norm.hip, token_logprobs.hip, grad_norm.hip): fp32, bf16 and fp16 in memory, fp32 arithmetic.
+//
+// Rows are read and written in 16-byte vectors wherever they start: the hardware takes 16-byte accesses at any element's address.
 #pragma once
 #include "bf16_common.h"
 
 __host__ __device__ constexpr int i2p_esize(int dtype) { return dtype == I2P_F32 ? 4 : 2; }
+__host__ __device__ constexpr int i2p_vec(int dtype) { return 16 / i2p_esize(dtype); }       // elements of a vector
+
+typedef _Float16 i2p_f16x2 __attribute__((ext_vector_type(2)));
 
 // one element
 template <int DT> __device__ __forceinline__ float ld1(const void *p, long long i) {
@@ -21,6 +26,73 @@ template <int DT> __device__ __forceinline__ void st1(void *p, long long i, floa
     else if constexpr (DT == I2P_BF16) reinterpret_cast<unsigned short *>(p)[i] = (unsigned short)bf_pack2(f, 0.f);
     else reinterpret_cast<_Float16 *>(p)[i] = (_Float16)f;
 }
+
+// a vector's values and back (round to nearest even)
+template <int DT> __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[i2p_vec(DT)]) {
+    if constexpr (DT == I2P_F32) { f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w); }
+    else if constexpr (DT == I2P_BF16) bf_unpack8(v, f);
+    else {
+        const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const i2p_f16x2 h = __builtin_bit_cast(i2p_f16x2, u[k]); f[2 * k] = (float)h.x; f[2 * k + 1] = (float)h.y; }
+    }
+}
+template <int DT> __device__ __forceinline__ uint4 pack(const float (&f)[i2p_vec(DT)]) {
+    if constexpr (DT == I2P_F32) return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    else if constexpr (DT == I2P_BF16) return bf_pack8(f);
+    else {
+        unsigned u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const i2p_f16x2 h = {(_Float16)f[2 * k], (_Float16)f[2 * k + 1]}; u[k] = __builtin_bit_cast(unsigned, h); }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+// Vector number `n` of a row of `d` elements.  The last, partial one is moved back so that it ends with the row: it reads and writes whole,
+// its first `skip` elements are the previous vector's (the same values, written twice), and are left out of sums.  A row shorter than a
+// vector (TINY) is read and written element by element instead.
+template <int DT, bool TINY = false> struct Col {
+    static constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT);
+    int at, skip;
+    bool in;
+    __device__ __forceinline__ Col(int n, int d) {
+        const int i = n * VE;
+        in = i < d;
+        at = TINY ? i : min(i, d - VE);
+        skip = TINY ? 0 : i - at;
+    }
+    __device__ __forceinline__ uint4 load(const char *row, int d) const {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (!in) return v;
+        if (!TINY || at + VE <= d) __builtin_memcpy(&v, row + (long long)at * ES, 16);
+        else {
+            unsigned u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (at + e < d) {
+                    if constexpr (ES == 4) u[e] = reinterpret_cast<const unsigned *>(row)[at + e];
+                    else u[e >> 1] |= (unsigned)reinterpret_cast<const unsigned short *>(row)[at + e] << (16 * (e & 1));
+                }
+            v = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        return v;
+    }
+    __device__ __forceinline__ void store(char *row, int d, const uint4 &v) const {
+        if (!in) return;
+        if (!TINY || at + VE <= d) __builtin_memcpy(row + (long long)at * ES, &v, 16);
+        else {
+            const unsigned u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (at + e < d) {
+                    if constexpr (ES == 4) reinterpret_cast<unsigned *>(row)[at + e] = u[e];
+                    else reinterpret_cast<unsigned short *>(row)[at + e] = (unsigned short)(u[e >> 1] >> (16 * (e & 1)));
+                }
+        }
+    }
+    // does element `e` of the vector count (is it the row's, and not the previous vector's)?
+    __device__ __forceinline__ bool counts(int e, int d) const { return in && e >= skip && (!TINY || at + e < d); }
+};
 
 // sum / maximum over the block's waves; every thread gets the result.  red: one float per wave.  (All threads of the block call it; the
 // trailing barrier lets the caller use `red` again.)
