@@ -102,7 +102,7 @@ template <class F> void for_tables(int n, const void *const *grads, const long l
     for (int i = 0; i < n; ++i)
         for (long long done = 0; done < numel[i]; done += PART) {
             const long long k = std::min(PART, numel[i] - done);
-            if (t.n == CAP || t.chunks + chunks_of(k) > 0x3fffffffll) { launch(t); t.n = t.chunks = 0; }
+            if (t.n == CAP || t.chunks + chunks_of(k) > (1 << 22)) { launch(t); t.n = t.chunks = 0; }
             const unsigned long long last = (unsigned long long)((k - 1) % CHUNK);
             t.ptr[t.n] = ((unsigned long long)grads[i] + (unsigned long long)done * i2p_esize(dtype[i])) | (last << 48);
             t.first[t.n] = t.chunks | ((unsigned)dtype[i] << 30);

@@ -350,11 +350,21 @@ template <class F, class G> void by_row(int dtype, int d, F f, G longer, int gro
 }
 
 template <bool Q8> int launch_fwd(int dtype, const FwdArgs &a, void *stream) {
-    if ((a.rows + 3) / 4 > 0x7fffffffll) return I2P_ERR_BAD_ARG;
     by_row(dtype, a.d, [&](auto dt, auto tpr, auto nv) {
         constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
-        hipLaunchKernelGGL((rms_fwd_kernel<dt.value, tpr.value, nv.value, Q8>), dim3((unsigned)((a.rows + RPB - 1) / RPB)), dim3(BLOCK), 0,
-                           (hipStream_t)stream, a);
+        constexpr long long MOST = 1ll << 21;                   // blocks of a launch: a grid has fewer than 2^32 threads
+        const long long es = i2p_esize(dt.value), ng = a.group ? (a.d + a.group - 1) / a.group : 1;
+        for (long long r = 0; r < a.rows; r += MOST * RPB) {
+            FwdArgs b = a;
+            b.rows = a.rows - r < MOST * RPB ? a.rows - r : MOST * RPB;
+            b.x += r * a.ldx * es;
+            if (a.res) { b.res += r * a.ldr * es; b.s += r * a.d * es; }
+            if (a.y) b.y += r * a.d * es;
+            if (a.rstd) b.rstd += r;
+            if (a.q) { b.q += r * a.d; b.scale += r * ng; }
+            hipLaunchKernelGGL((rms_fwd_kernel<dt.value, tpr.value, nv.value, Q8>), dim3((unsigned)((b.rows + RPB - 1) / RPB)), dim3(BLOCK), 0,
+                               (hipStream_t)stream, b);
+        }
     }, [&](auto dt) {
         hipLaunchKernelGGL((rms_fwd_long_kernel<dt.value, Q8>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), dim3(LT), 0,
                            (hipStream_t)stream, a);
@@ -368,7 +378,7 @@ extern "C" int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, co
                                 const void *w, float eps, void *s, void *y, float *rstd, void *stream) {
     if (rows < 0 || d <= 0 || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
-    if (!x || !y || rows > 0x7fffffffll) return I2P_ERR_BAD_ARG;
+    if (!x || !y) return I2P_ERR_BAD_ARG;
     return launch_fwd<false>(dtype, FwdArgs{rows, d, wdtype, (const char *)x, ldx, (const char *)res, ldr, w, eps, (char *)s, (char *)y, rstd, 0,
                                             nullptr, nullptr}, stream);
 }
@@ -378,7 +388,7 @@ extern "C" int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, con
     if (rows < 0 || d <= 0 || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
     if (group != 0 && (group < 32 || group > 512 || (group & (group - 1)))) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
-    if (!x || !q || !scale || rows > 0x7fffffffll) return I2P_ERR_BAD_ARG;
+    if (!x || !q || !scale) return I2P_ERR_BAD_ARG;
     return launch_fwd<true>(dtype, FwdArgs{rows, d, wdtype, (const char *)x, ldx, (const char *)res, ldr, w, eps, (char *)s, nullptr, nullptr, group,
                                            q, scale}, stream);
 }

@@ -5,13 +5,21 @@
 //
 // The maximum and L are kept apart for the backward pass: rounded into one number, scores of a few hundred would lose the digits of L.
 // A row without candidates (all -inf): logp -inf, H 0, gradient 0.  +inf or NaN in a row: logp, H, top_logp and the gradient are NaN.
+//
+// Forward: bound by the one read of the scores.  A row, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at
+// most 32 scores a thread), so that the true maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k best
+// in the workspace and a second launch joins them.
+// Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those is a value that at least k scores reach and that
+// few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow that list
+// and are searched k times instead.
 #include "rows_common.h"
 
 namespace {
 
-constexpr int T = 256;
+constexpr int LIST = 256;                       // scores ranked by counting
 
 // order of the alternatives: by value, NaN above +inf, -0 equal to +0; then by lower index.  0 is below every key
+typedef unsigned long long skey;
 __device__ __forceinline__ unsigned order_of(float x) {
     x += 0.f;
     if (x != x) return 0xffc00000u;
@@ -19,80 +27,282 @@ __device__ __forceinline__ unsigned order_of(float x) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
-__device__ __forceinline__ unsigned long long key_of(float x, unsigned col) { return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - col); }
+__device__ __forceinline__ skey key_of(float x, unsigned col) { return ((skey)order_of(x) << 32) | (0xffffffffu - col); }
+__device__ __forceinline__ float score_of(skey k) { return value_of((unsigned)(k >> 32)); }
+__device__ __forceinline__ int64_t col_of(skey k) { return (int64_t)(0xffffffffu - (unsigned)k); }
 
 __device__ __forceinline__ float shift_of(float m) { return m == -__builtin_inff() ? 0.f : m; }
-// z e^z with 0 in the limit z -> -inf
-__device__ __forceinline__ float z_exp(float z, float e) { return fmaxf(z, -200.f) * e; }      // (e^-200 is 0)
+// z e^z with 0 in the limit z -> -inf (e^-200 is 0)
+__device__ __forceinline__ float z_exp(float z, float e, float acc) { return __builtin_fmaf(fmaxf(z, -200.f), e, acc); }
 
-template <int DT>
-__global__ __launch_bounds__(T) void logprobs_fwd_kernel(long long rows, int v, const void *__restrict__ x, long long ldx,
-                                                         const int64_t *__restrict__ ids, long long ignore, int top, float *__restrict__ logp,
-                                                         float *__restrict__ entropy, float *__restrict__ stat, float *__restrict__ top_logp,
-                                                         int64_t *__restrict__ top_ids) {
-    __shared__ float red[T / 64];
-    __shared__ unsigned long long kred[T / 64];
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        const long long id = ids[row], base = row * ldx;
-        if (id == ignore) {
-            if (threadIdx.x == 0) { logp[row] = 0.f; entropy[row] = 0.f; stat[2 * row] = 0.f; stat[2 * row + 1] = 0.f; }
-            for (int k = threadIdx.x; k < top; k += T) { top_logp[row * top + k] = -__builtin_inff(); top_ids[row * top + k] = -1; }
-            continue;
-        }
-        float m = -__builtin_inff();
-        for (int i = threadIdx.x; i < v; i += T) m = fmaxf(m, ld1<DT>(x, base + i));
-        m = block_reduce<true>(m, red);
-        const float c = shift_of(m);
-        float S = 0.f, U = 0.f;
-        for (int i = threadIdx.x; i < v; i += T) { const float z = ld1<DT>(x, base + i) - c, e = __expf(z); S += e; U += z_exp(z, e); }
-        S = block_reduce<false>(S, red);
-        U = block_reduce<false>(U, red);
-        const bool empty = S == 0.f;
-        const float L = empty ? __builtin_inff() : logf(S);
-        if (threadIdx.x == 0) {
-            logp[row] = id < 0 || id >= v ? __builtin_nanf("") : (ld1<DT>(x, base + id) - c) - L;
-            entropy[row] = empty ? 0.f : L - U / S;
-            stat[2 * row] = c; stat[2 * row + 1] = L;
-        }
-        unsigned long long last = ~0ull;
-        for (int k = 0; k < top; ++k) {
-            unsigned long long best = 0;
-            for (int i = threadIdx.x; i < v; i += T) { const unsigned long long key = key_of(ld1<DT>(x, base + i), i); if (key < last && key > best) best = key; }
+struct FwdArgs {
+    long long rows; int v; const char *x; long long ldx; const int64_t *ids; long long ignore; int top; float *logp, *entropy, *stat, *top_logp;
+    int64_t *top_ids;
+    int nsplit, slice;                          // slices of a row, scores of a slice
+    float4 *part;                               // [rows][nsplit]: max, S, sum z e^z
+    skey *keys;                                // [rows][nsplit][top], best first
+};
+
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) { const unsigned long long u = __shfl_xor(best, o, 64); best = u > best ? u : best; }
-            if ((threadIdx.x & 63) == 0) kred[threadIdx.x >> 6] = best;
-            __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
-            for (int wv = 0; wv < T / 64; ++wv) best = kred[wv] > best ? kred[wv] : best;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                top_logp[row * top + k] = (value_of((unsigned)(best >> 32)) - c) - L;
-                top_ids[row * top + k] = (int64_t)(0xffffffffu - (unsigned)best);
-            }
-            last = best;
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// what a row's results are, from its maximum and sums; one thread
+__device__ __forceinline__ void finish_row(const FwdArgs &a, long long row, long long id, float xid, float c, float S, float U) {
+    const bool empty = S == 0.f;
+    const float L = empty ? __builtin_inff() : logf(S);
+    a.logp[row] = id < 0 || id >= a.v ? __builtin_nanf("") : (xid - c) - L;
+    a.entropy[row] = empty ? 0.f : L - U / S;
+    a.stat[2 * row] = c; a.stat[2 * row + 1] = L;
+}
+__device__ __forceinline__ void put_top(const FwdArgs &a, long long row, int rank, skey key, float c, float S) {
+    a.top_logp[row * a.top + rank] = S == 0.f ? -__builtin_inff() : (score_of(key) - c) - logf(S);
+    a.top_ids[row * a.top + rank] = col_of(key);
+}
+__device__ __forceinline__ void skip_row(const FwdArgs &a, long long row) {
+    if (threadIdx.x == 0) { a.logp[row] = 0.f; a.entropy[row] = 0.f; a.stat[2 * row] = 0.f; a.stat[2 * row + 1] = 0.f; }
+    for (int k = threadIdx.x; k < a.top; k += blockDim.x) { a.top_logp[row * a.top + k] = -__builtin_inff(); a.top_ids[row * a.top + k] = -1; }
+}
+
+template <int DT> __device__ __forceinline__ constexpr unsigned minus_inf() { return DT == I2P_F32 ? 0xff800000u : DT == I2P_BF16 ? 0xff80ff80u : 0xfc00fc00u; }
+
+// keeps the scores packed between the phases: the compiler would hold their fp32 values, and half as many waves would fit
+template <int N> __device__ __forceinline__ void hold(uint4 (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) asm volatile("" : "+v"(v[j].x), "+v"(v[j].y), "+v"(v[j].z), "+v"(v[j].w));
+}
+
+template <int DT, int W, int E>
+__global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8) void logprobs_fwd_kernel(FwdArgs a) {
+    constexpr int T = 64 * W, VE = i2p_vec(DT), NV = E / VE;
+    constexpr bool TINY = T * E == 512;
+    __shared__ float gmax[64], sums[2][W], bound;
+    __shared__ skey list[LIST], best[W];
+    __shared__ int count;
+    const long long row = blockIdx.x / (unsigned)a.nsplit;      // (one row's slices stay together)
+    const int part = (int)(blockIdx.x - (unsigned)row * (unsigned)a.nsplit), lo = part * a.slice, n = min(a.slice, a.v - lo);
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const long long id = a.ids[row];
+    const char *x = a.x + (row * a.ldx + lo) * i2p_esize(DT);
+    if (id == a.ignore) { if (a.nsplit == 1) skip_row(a, row); return; }
+    uint4 v[NV];
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const Col<DT, TINY> c(j * T + t, n);
+        v[j] = c.load(x, n);
+        if (!c.in || c.skip || c.at + VE > n) {                 // what is not this vector's reads as -inf
+            float f[VE];
+            unpack<DT>(v[j], f);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[e] = c.counts(e, n) ? f[e] : -__builtin_inff();
+            v[j] = pack<DT>(f);
         }
+    }
+    float xid = 0.f;
+    if (a.nsplit == 1 && t == 0 && id >= 0 && id < a.v) xid = ld1<DT>(x, id);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float f[VE];
+        unpack<DT>(v[j], f);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) most = fmaxf(most, f[e]);
+    }
+    hold(v);
+    // 64 groups of W lanes
+    float g = most;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor(g, o, 64));
+    if constexpr (W > 1) {
+        if ((t & (W - 1)) == 0) gmax[t / W] = g;
+        if (t == 0) count = 0;
+        __syncthreads();
+        g = gmax[lane];
+    } else if (t == 0) count = 0;
+    const float m = wave_max(g), c = shift_of(m);
+    if (a.top) {                                                // each wave ranks 64 / W of the groups
+#pragma unroll 4
+        for (int i = 0; i < 64 / W; ++i) {
+            const int k = __builtin_amdgcn_readfirstlane(wave) * (64 / W) + i;
+            const float gk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), k));
+            const skey above = __ballot(g > gk), equal = __ballot(g == gk) & ((1ull << k) - 1ull);
+            if (__popcll(above) + __popcll(equal) == a.top - 1 && lane == 0) bound = gk;
+        }
+    }
+    float S = 0.f, U = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float f[VE];
+        unpack<DT>(v[j], f);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) { const float z = f[e] - c, ez = __expf(z); S += ez; U = z_exp(z, ez, U); }
+    }
+    hold(v);
+    S = wave_sum(S); U = wave_sum(U);
+    if constexpr (W > 1) {
+        if (lane == 0) { sums[0][wave] = S; sums[1][wave] = U; }
+        __syncthreads();
+        S = U = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) { S += sums[0][w]; U += sums[1][w]; }
+    }
+    if (t == 0) {
+        if (a.nsplit == 1) finish_row(a, row, id, xid, c, S, U);
+        else a.part[row * a.nsplit + part] = make_float4(m, S, U, 0.f);
+    }
+    if (!a.top) return;
+    auto put = [&](int rank, skey key) {
+        if (a.nsplit == 1) put_top(a, row, rank, key, c, S);
+        else a.keys[(row * a.nsplit + part) * a.top + rank] = key;
+    };
+    if constexpr (W == 1) __syncthreads();                      // (`bound`, `count`)
+    const float least = bound;
+    const bool plain = S == S;                                  // no NaN, no +inf
+    if (plain && most >= least) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const Col<DT, TINY> col(j * T + t, n);
+            float f[VE];
+            unpack<DT>(v[j], f);
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (f[e] >= least && col.counts(e, n)) {
+                    const int at = atomicAdd(&count, 1);
+                    if (at < LIST) list[at] = key_of(f[e], (unsigned)(lo + col.at + e));
+                }
+        }
+    }
+    __syncthreads();
+    const int found = count;
+    if (plain && found <= LIST) {
+        for (int i = t; i < found; i += T) {
+            const skey key = list[i];
+            int rank = 0;
+            for (int k = 0; k < found; ++k) rank += list[k] > key;
+            if (rank < a.top) put(rank, key);
+        }
+        return;
+    }
+    skey last = ~0ull;                                          // (rare: the scores are read again, from the caches)
+    for (int k = 0; k < a.top; ++k) {
+        skey top = 0;
+        for (int i = t; i < n; i += T) {
+            const skey key = key_of(ld1<DT>(x, i), (unsigned)(lo + i));
+            if (key < last && key > top) top = key;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) { const skey u = __shfl_xor(top, o, 64); top = u > top ? u : top; }
+        if (lane == 0) best[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = best[w] > top ? best[w] : top;
+        __syncthreads();
+        if (t == 0) put(k, top);
+        last = top;
     }
 }
 
-template <int DT>
-__global__ __launch_bounds__(T) void logprobs_bwd_kernel(long long rows, int v, const void *__restrict__ x, long long ldx,
-                                                         const int64_t *__restrict__ ids, long long ignore, const float *__restrict__ stat,
-                                                         const float *__restrict__ entropy, const float *__restrict__ g_logp,
-                                                         const float *__restrict__ g_entropy, void *__restrict__ dx) {
-    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-        const long long id = ids[row];
-        const bool skip = id == ignore;
-        float gl = g_logp ? g_logp[row] : 0.f;
-        const float gh = g_entropy ? g_entropy[row] : 0.f, H = entropy[row], c = stat[2 * row], L = stat[2 * row + 1];
-        if (L == __builtin_inff()) gl = 0.f;                 // an empty row
-        if (id < 0 || id >= v) gl = __builtin_nanf("");
-        for (int i = threadIdx.x; i < v; i += T) {
-            float g = 0.f;
-            if (!skip) {
-                const float lp = ld1<DT>(x, row * ldx + i) - c - L, p = __expf(lp);
-                g = (i == id ? gl : 0.f) - p * (gl + gh * (fmaxf(lp, -200.f) + H));
+// Joins the slices of a row.  The k-th largest of the slices' best keys bounds the row's k best from below; a slice's keys are in order
+constexpr int JT = 256;                         // = most slices of a row
+__global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype) {
+    __shared__ float sums[3][JT / 64];
+    __shared__ skey head[JT], list[I2P_MAX_TOP * I2P_MAX_TOP], bound;
+    __shared__ int count;
+    const long long row = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const long long id = a.ids[row];
+    if (id == a.ignore) { skip_row(a, row); return; }
+    const float4 p = t < a.nsplit ? a.part[row * a.nsplit + t] : make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
+    const skey *keys = a.keys + (row * a.nsplit + t) * a.top;
+    const skey mine = a.top && t < a.nsplit ? keys[0] : 0ull;
+    float xid = 0.f;
+    if (t == 0 && id >= 0 && id < a.v) {
+        const long long i = row * a.ldx + id;
+        xid = dtype == I2P_F32 ? ld1<I2P_F32>(a.x, i) : dtype == I2P_BF16 ? ld1<I2P_BF16>(a.x, i) : ld1<I2P_F16>(a.x, i);
+    }
+    float m = wave_max(p.x);
+    if (lane == 0) sums[0][wave] = m;
+    head[t] = mine;
+    if (t == 0) { count = 0; bound = 0ull; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < JT / 64; ++w) m = fmaxf(m, sums[0][w]);
+    const float c = shift_of(m), shift = p.x - c, f = __expf(shift);
+    float S = wave_sum(f * p.y), U = wave_sum(f * __builtin_fmaf(fmaxf(shift, -200.f), p.y, p.z));
+    if (lane == 0) { sums[1][wave] = S; sums[2][wave] = U; }
+    if (a.top && t < a.nsplit) {
+        int rank = 0;
+        for (int k = 0; k < a.nsplit; ++k) rank += head[k] > mine;
+        if (rank == a.top - 1) bound = mine;
+    }
+    __syncthreads();
+    S = U = 0.f;
+#pragma unroll
+    for (int w = 0; w < JT / 64; ++w) { S += sums[1][w]; U += sums[2][w]; }
+    if (t == 0) finish_row(a, row, id, xid, c, S, U);
+    if (!a.top) return;
+    if (t < a.nsplit && mine >= bound)
+        for (int k = 0; k < a.top; ++k) {                       // (at most `top` slices reach the bound, unless there are fewer slices)
+            const skey key = keys[k];
+            if (key < bound) break;
+            list[atomicAdd(&count, 1)] = key;
+        }
+    __syncthreads();
+    const int found = count;
+    for (int i = t; i < found; i += JT) {
+        const skey key = list[i];
+        int rank = 0;
+        for (int k = 0; k < found; ++k) rank += list[k] > key;
+        if (rank < a.top) put_top(a, row, rank, key, c, S);
+    }
+}
+
+struct BwdArgs {
+    long long rows; int v; const char *x; long long ldx; const int64_t *ids; long long ignore; const float *stat, *entropy, *g_logp, *g_entropy;
+    char *dx; int pieces;                       // pieces of a row, each BV vectors of the TPR threads that share it
+};
+constexpr int BV = 4;
+
+template <int DT, int TPR>
+__global__ __launch_bounds__(256) void logprobs_bwd_kernel(BwdArgs a) {
+    constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT);
+    constexpr bool TINY = TPR == 16;
+    const long long work = a.rows * a.pieces;
+    const int t = threadIdx.x % TPR;
+    for (long long i = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR; i < work; i += (long long)gridDim.x * (256 / TPR)) {
+        const long long row = a.pieces == 1 ? i : i / a.pieces;
+        const int piece = (int)(i - row * a.pieces);
+        const char *x = a.x + row * a.ldx * ES;
+        const long long id = a.ids[row];
+        uint4 u[BV];
+        if (id != a.ignore)
+#pragma unroll
+            for (int j = 0; j < BV; ++j) u[j] = Col<DT, TINY>((piece * BV + j) * TPR + t, a.v).load(x, a.v);
+        const float gh = a.g_entropy ? a.g_entropy[row] : 0.f, H = a.entropy[row], c = a.stat[2 * row], L = a.stat[2 * row + 1];
+        float gl = a.g_logp ? a.g_logp[row] : 0.f;
+        if (L == __builtin_inff()) gl = 0.f;                     // an empty row
+        if (id < 0 || id >= a.v) gl = __builtin_nanf("");
+#pragma unroll
+        for (int j = 0; j < BV; ++j) {
+            const Col<DT, TINY> col((piece * BV + j) * TPR + t, a.v);
+            if (!col.in) break;
+            float f[VE] = {};
+            if (id != a.ignore) {
+                unpack<DT>(u[j], f);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    const float lp = f[e] - c - L, p = __expf(lp);
+                    f[e] = (col.at + e == id ? gl : 0.f) - p * __builtin_fmaf(gh, fmaxf(lp, -200.f) + H, gl);
+                }
             }
-            st1<DT>(dx, row * v + i, g);
+            col.store(a.dx + row * a.v * ES, a.v, pack<DT>(f));
         }
     }
 }
@@ -103,33 +313,76 @@ template <class F> void by_type(int dtype, F f) {
     else f(std::integral_constant<int, I2P_F16>{});
 }
 
+constexpr int WHOLE = 32768;                    // scores that 16 waves hold
+constexpr int SLICE = 8192;                     // 4 waves
+
+// how a row is cut: one block up to 32768 scores; longer rows in slices of at most that, or of at most 8192 where few rows would leave most
+// of the 256 CUs without one
+inline void cut(long long rows, int v, int &nsplit, int &slice) {
+    nsplit = (v + WHOLE - 1) / WHOLE;
+    if (nsplit > 1 && rows * nsplit < 256) nsplit = (v + SLICE - 1) / SLICE;
+    slice = ((v + nsplit - 1) / nsplit + 7) & ~7;
+    nsplit = (v + slice - 1) / slice;
+}
+
+inline bool sizes_ok(long long rows, int v, int dtype, long long ldx) {
+    return rows >= 0 && v > 0 && v <= I2P_MAX_CANDIDATES && dtype >= I2P_F32 && dtype <= I2P_F16 && ldx >= v;
+}
+
 }  // namespace
 
-extern "C" long long i2p_token_logprobs_scratch(long long, int, int, int) { return 0; }
+extern "C" long long i2p_token_logprobs_scratch(long long rows, int v, int, int top) {
+    if (rows <= 0 || v <= 0 || v > I2P_MAX_CANDIDATES || top < 0 || top > I2P_MAX_TOP) return 0;
+    int nsplit, slice;
+    cut(rows, v, nsplit, slice);
+    return nsplit == 1 ? 0 : rows * nsplit * (16 + 8ll * top);
+}
 
 extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const void *x, long long ldx, const int64_t *ids, long long ignore, int top,
-                                      float *logp, float *entropy, float *stat, float *top_logp, int64_t *top_ids, void *scratch,
-                                      void *stream) {
-    if (rows < 0 || v <= 0 || v > I2P_MAX_CANDIDATES || dtype < I2P_F32 || dtype > I2P_F16 || ldx < v || top < 0 || top > v || top > I2P_MAX_TOP) return I2P_ERR_BAD_ARG;
+                                      float *logp, float *entropy, float *stat, float *top_logp, int64_t *top_ids, void *scratch, void *stream) {
+    if (!sizes_ok(rows, v, dtype, ldx) || top < 0 || top > v || top > I2P_MAX_TOP) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
     if (!x || !ids || !logp || !entropy || !stat || (top && (!top_logp || !top_ids))) return I2P_ERR_BAD_ARG;
-    const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : (1 << 20));
-    by_type(dtype, [&](auto dt) {
-        hipLaunchKernelGGL((logprobs_fwd_kernel<dt.value>), dim3(grid), dim3(T), 0, (hipStream_t)stream, rows, v, x, ldx, ids, ignore, top, logp,
-                           entropy, stat, top_logp, top_ids);
+    int nsplit, slice;
+    cut(rows, v, nsplit, slice);
+    if (nsplit > 1 && !scratch) return I2P_ERR_BAD_ARG;
+    hipStream_t st = (hipStream_t)stream;
+    const long long most = (1 << 21) / nsplit;                  // rows of a launch: a grid has fewer than 2^32 threads
+    for (long long r = 0; r < rows; r += most) by_type(dtype, [&](auto dt) {
+        const long long k = rows - r < most ? rows - r : most;
+        const FwdArgs a{k, v, (const char *)x + r * ldx * i2p_esize(dtype), ldx, ids + r, ignore, top, logp + r, entropy + r, stat + 2 * r,
+                        top_logp + r * top, top_ids + r * top, nsplit, slice, (float4 *)scratch + r * nsplit,
+                        (skey *)((char *)scratch + rows * nsplit * 16) + r * nsplit * top};
+        const dim3 grid((unsigned)(k * nsplit));
+        constexpr int DT = dt.value;
+        if (slice <= 512) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 8>), grid, dim3(64), 0, st, a);
+        else if (slice <= 2048) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 32>), grid, dim3(64), 0, st, a);
+        else if (slice <= 4096) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 16>), grid, dim3(256), 0, st, a);
+        else if (slice <= SLICE) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 32>), grid, dim3(256), 0, st, a);
+        else if (slice <= 16384) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 16, 16>), grid, dim3(1024), 0, st, a);
+        else hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 16, 32>), grid, dim3(1024), 0, st, a);
+        if (nsplit > 1) hipLaunchKernelGGL(logprobs_join_kernel, dim3((unsigned)k), dim3(JT), 0, st, a, dtype);
     });
     I2P_RETURN_LAUNCH_STATUS();
 }
 
 extern "C" int i2p_token_logprobs_bwd(long long rows, int v, int dtype, const void *x, long long ldx, const int64_t *ids, long long ignore,
                                       const float *stat, const float *entropy, const float *g_logp, const float *g_entropy, void *dx, void *stream) {
-    if (rows < 0 || v <= 0 || v > I2P_MAX_CANDIDATES || dtype < I2P_F32 || dtype > I2P_F16 || ldx < v) return I2P_ERR_BAD_ARG;
+    if (!sizes_ok(rows, v, dtype, ldx)) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
     if (!x || !ids || !stat || !entropy || !dx) return I2P_ERR_BAD_ARG;
-    const unsigned grid = (unsigned)(rows < (1 << 20) ? rows : (1 << 20));
     by_type(dtype, [&](auto dt) {
-        hipLaunchKernelGGL((logprobs_bwd_kernel<dt.value>), dim3(grid), dim3(T), 0, (hipStream_t)stream, rows, v, x, ldx, ids, ignore, stat, entropy,
-                           g_logp, g_entropy, dx);
+        constexpr int DT = dt.value;
+        const int nvec = (v + i2p_vec(DT) - 1) / i2p_vec(DT);
+        auto go = [&](auto tpr) {
+            constexpr int TPR = tpr.value;
+            const BwdArgs a{rows, v, (const char *)x, ldx, ids, ignore, stat, entropy, g_logp, g_entropy, (char *)dx, (nvec + TPR * BV - 1) / (TPR * BV)};
+            const long long blocks = (rows * a.pieces + 256 / TPR - 1) / (256 / TPR);
+            hipLaunchKernelGGL((logprobs_bwd_kernel<DT, TPR>), dim3((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22))), dim3(256), 0, (hipStream_t)stream, a);
+        };
+        if (nvec <= 16 * BV) go(std::integral_constant<int, 16>{});
+        else if (nvec <= 64 * BV) go(std::integral_constant<int, 64>{});
+        else go(std::integral_constant<int, 256>{});
     });
     I2P_RETURN_LAUNCH_STATUS();
 }

@@ -49,6 +49,12 @@ def test_token_logprobs_refusals(change):
         call("i2p_token_logprobs_fwd", *a.values())
 
 
+def test_token_logprobs_needs_its_scratch():
+    assert _lib.helper("i2p_token_logprobs_scratch", 1, 1 << 20, 0, 0) > 0 and _lib.helper("i2p_token_logprobs_scratch", 1, 1000, 0, 32) == 0
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_token_logprobs_fwd", 1, 1 << 20, 0, P, 1 << 20, P, -100, 0, P, P, P, P, P, None)
+
+
 @pytest.mark.parametrize("change", [dict(v=0), dict(dtype=3), dict(ldx=3), dict(x=None), dict(ids=None), dict(stat=None), dict(entropy=None), dict(dx=None)])
 def test_token_logprobs_backward_refusals(change):
     a = dict(rows=2, v=8, dtype=1, x=P, ldx=8, ids=P, ignore=-100, stat=P, entropy=P, gl=None, gh=None, dx=P) | change

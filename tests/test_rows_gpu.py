@@ -215,6 +215,21 @@ def test_rms_norm_extremes():
     assert torch.equal(half.cpu(), torch.ones(1, 8, dtype=torch.float16))
 
 
+def test_more_rows_than_one_launch_takes():
+    rows = (1 << 25) + 77                       # 16 rows a block, 2^21 blocks a launch
+    x = torch.full((rows, 1), 3.0, dtype=torch.bfloat16, device=DEV)
+    x[-1] = -3.0
+    x[1 << 25] = 0.0
+    y, s = modules.rms_norm(x, None, residual=x)
+    assert s[-1] == -6 and y[-1] == -1 and y[1 << 25] == 0 and y[(1 << 25) - 1] == 1 and int(y.eq(1).sum()) == rows - 2
+    q, scale = modules.rms_norm_q8(x, None)
+    assert q[-1].float() == -448 and scale[-1] > 0 and scale[1 << 25] == 1
+    ids = torch.zeros(rows, dtype=torch.long, device=DEV)
+    ids[-1] = 5
+    o = loss.token_logprobs(x, ids, top=1)      # 2^21 rows a launch
+    assert torch.isnan(o.logp[-1]) and not o.logp[:-1].any() and not o.entropy.any() and not o.top_ids.any() and not o.top_logp.any()
+
+
 # ---- log probabilities -----------------------------------------------------------------------------------------------------------
 def logp64(x, ids, top, gl=None, gh=None):
     a = x.double()
