@@ -50,12 +50,33 @@ template <bool MAX> __device__ __forceinline__ double block_sum(double v, double
     return t;
 }
 
-template <int DT, bool MAX> __device__ __forceinline__ double norm_piece(const Piece &p) {
-    double acc = 0.0;
-    for (unsigned i = threadIdx.x; i < p.count; i += T) {
-        const double g = (double)ld1<DT>((const void *)p.p, i);
-        acc = MAX ? nan_max(acc, fabs(g)) : acc + g * g;
+// A piece is read in 16-byte vectors from wherever it starts, BATCH of a thread in flight; its last elements one by one
+constexpr int BATCH = 4;
+template <int DT, class F> __device__ __forceinline__ void for_vectors(const Piece &p, F f) {
+    constexpr int VE = i2p_vec(DT);
+    const char *base = (const char *)p.p;
+    const unsigned nv = p.count / VE;
+    for (unsigned v0 = threadIdx.x; v0 < nv; v0 += BATCH * T) {
+        uint4 u[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (v0 + j * T < nv) __builtin_memcpy(&u[j], base + (size_t)(v0 + j * T) * 16, 16);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (v0 + j * T < nv) { float g[VE]; unpack<DT>(u[j], g); f(g, (v0 + j * T) * VE); }
     }
+}
+
+template <int DT, bool MAX> __device__ __forceinline__ double norm_piece(const Piece &p) {
+    constexpr int VE = i2p_vec(DT);
+    double acc = 0.0;
+    auto add = [&](float g) { acc = MAX ? nan_max(acc, (double)fabsf(g)) : __builtin_fma((double)g, (double)g, acc); };
+    for_vectors<DT>(p, [&](const float (&g)[VE], unsigned) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) add(g[e]);
+    });
+    const unsigned rest = p.count / VE * VE + threadIdx.x;
+    if (rest < p.count) add(ld1<DT>((const void *)p.p, rest));
     return acc;
 }
 
@@ -76,10 +97,19 @@ template <bool MAX> __global__ __launch_bounds__(1024) void grad_total_kernel(un
 }
 
 template <int DT> __device__ __forceinline__ void clip_piece(const Piece &p, float c, float *out) {
-    for (unsigned i = threadIdx.x; i < p.count; i += T) {
-        const float g = ld1<DT>((const void *)p.p, i) * c;
-        if (out) out[p.off + i] = g;
-        else st1<DT>((void *)p.p, i, g);
+    constexpr int VE = i2p_vec(DT);
+    for_vectors<DT>(p, [&](const float (&g)[VE], unsigned i) {
+        float h[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) h[e] = g[e] * c;
+        if (out) __builtin_memcpy(out + p.off + i, h, 4 * VE);
+        else { const uint4 u = pack<DT>(h); __builtin_memcpy((char *)p.p + (size_t)i * i2p_esize(DT), &u, 16); }
+    });
+    const unsigned rest = p.count / VE * VE + threadIdx.x;
+    if (rest < p.count) {
+        const float g = ld1<DT>((const void *)p.p, rest) * c;
+        if (out) out[p.off + rest] = g;
+        else st1<DT>((void *)p.p, rest, g);
     }
 }
 
