@@ -10,6 +10,7 @@
 // rows per block), longer ones by a block of 256 or 1024.  Sums are fp32; dw is summed per block over the rows it owns (fp32 registers),
 // then over the blocks in index order: reproducible.
 #include "rows_common.h"
+#include <algorithm>
 
 namespace {
 
@@ -61,10 +62,9 @@ __device__ __forceinline__ float scale_of(unsigned bits) {
     return sc < 1.17549435e-38f ? 1.f : sc;
 }
 
-template <int DT, int TPR, int NV, bool Q8>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(FwdArgs a) {
+template <int DT, int TPR, int NV, bool TINY, bool Q8>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4) void rms_fwd_kernel(FwdArgs a) {
     constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT), BLOCK = TPR < 256 ? 256 : TPR;
-    constexpr bool TINY = TPR == 16;
     __shared__ float red[TPR > 64 ? TPR / 64 : 1];
     __shared__ unsigned mred[TPR > 64 ? TPR / 64 : 1];
     const long long row = (long long)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
@@ -163,10 +163,9 @@ struct BwdArgs {
 };
 
 // Every group of TPR threads walks rows in steps of the grid
-template <int DT, int TPR, int NV>
+template <int DT, int TPR, int NV, bool TINY>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(BwdArgs a) {
     constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
-    constexpr bool TINY = TPR == 16;
     __shared__ float red[2][TPR > 64 ? TPR / 64 : 1];
     __shared__ float cols[RPB > 1 ? BLOCK * VE : 1];
     const int t = threadIdx.x % TPR, d = a.d;
@@ -237,8 +236,10 @@ __global__ __launch_bounds__(DW_COLS * DW_LANES) void rms_dw_kernel(int nblk, in
     const int c = threadIdx.x % DW_COLS, l = threadIdx.x / DW_COLS, i = blockIdx.x * DW_COLS + c;
     float v = 0.f;
     if (i < d)
-#pragma unroll 4
-        for (int b = l; b < nblk; b += DW_LANES) v += part[(long long)b * d + i];
+        for (int b = l; b < nblk; b += 16 * DW_LANES) {          // 16 loads in flight
+#pragma unroll
+            for (int u = 0; u < 16; ++u) { const int k = b + u * DW_LANES; v += k < nblk ? part[(long long)k * d + i] : 0.f; }
+        }
     sum[l][c] = v;
     __syncthreads();
     if (l || i >= d) return;
@@ -330,15 +331,31 @@ inline bool types_ok(int dtype, int wdtype) {
     return dtype >= I2P_F32 && dtype <= I2P_F16 && (wdtype == I2P_F32 || wdtype == dtype);
 }
 
-constexpr long long BWD_BLOCKS = 512;
-inline long long bwd_blocks(long long rows) { return rows < BWD_BLOCKS ? rows : BWD_BLOCKS; }
+// Blocks of the backward pass for `rows` rows (or runs of rows) of a block of `threads`: as many as run at once (four waves a SIMD), but no
+// more than 2^21 partial weight gradients, whose write and read cost as much as a row's (8192 x 4096 bf16: 512 blocks 59 us, 1024 61, 2048 75;
+// 30000 x 1000: 512 blocks 46 us, 1024 44, 2048 48)
+inline long long bwd_blocks(long long rows, int d, int threads) {
+    const long long most = std::min(262144ll / threads, std::max(256ll, (1ll << 21) / d));
+    return std::min(rows, most);
+}
 
 // f(DT, TPR, NV) for rows of d elements; false: the row does not fit the registers of a block
 template <int DT, class F> bool by_width(int d, F f) {
     using std::integral_constant;
     const long long n = ((long long)d + i2p_vec(DT) - 1) / i2p_vec(DT);
-#define I2P_ROW(TPR, NV) if (n <= (TPR) * (NV)) { f(integral_constant<int, DT>{}, integral_constant<int, TPR>{}, integral_constant<int, NV>{}); return true; }
-    I2P_ROW(16, 1) I2P_ROW(64, 1) I2P_ROW(64, 2) I2P_ROW(256, 1) I2P_ROW(256, 2) I2P_ROW(256, 4) I2P_ROW(1024, 2) I2P_ROW(1024, 4)
+#define I2P_ROW(TPR, NV, TINY) { f(integral_constant<int, DT>{}, integral_constant<int, TPR>{}, integral_constant<int, NV>{}, std::bool_constant<TINY>{}); return true; }
+    if (d < i2p_vec(DT)) I2P_ROW(8, 1, true)
+    if (n <= 8) I2P_ROW(8, 1, false)
+    if (n <= 16) I2P_ROW(16, 1, false)
+    if (n <= 32) I2P_ROW(16, 2, false)
+    if (n <= 64) I2P_ROW(64, 1, false)
+    if (n <= 128) I2P_ROW(64, 2, false)
+    if (n <= 256) I2P_ROW(256, 1, false)
+    if (n <= 512) I2P_ROW(256, 2, false)
+    if (n <= 768) I2P_ROW(256, 3, false)
+    if (n <= 1024) I2P_ROW(512, 2, false)
+    if (n <= 2048) I2P_ROW(1024, 2, false)
+    if (n <= 4096) I2P_ROW(1024, 4, false)
 #undef I2P_ROW
     return false;
 }
@@ -350,7 +367,7 @@ template <class F, class G> void by_row(int dtype, int d, F f, G longer, int gro
 }
 
 template <bool Q8> int launch_fwd(int dtype, const FwdArgs &a, void *stream) {
-    by_row(dtype, a.d, [&](auto dt, auto tpr, auto nv) {
+    by_row(dtype, a.d, [&](auto dt, auto tpr, auto nv, auto tiny) {
         constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
         constexpr long long MOST = 1ll << 21;                   // blocks of a launch: a grid has fewer than 2^32 threads
         const long long es = i2p_esize(dt.value), ng = a.group ? (a.d + a.group - 1) / a.group : 1;
@@ -362,7 +379,7 @@ template <bool Q8> int launch_fwd(int dtype, const FwdArgs &a, void *stream) {
             if (a.y) b.y += r * a.d * es;
             if (a.rstd) b.rstd += r;
             if (a.q) { b.q += r * a.d; b.scale += r * ng; }
-            hipLaunchKernelGGL((rms_fwd_kernel<dt.value, tpr.value, nv.value, Q8>), dim3((unsigned)((b.rows + RPB - 1) / RPB)), dim3(BLOCK), 0,
+            hipLaunchKernelGGL((rms_fwd_kernel<dt.value, tpr.value, nv.value, tiny.value, Q8>), dim3((unsigned)((b.rows + RPB - 1) / RPB)), dim3(BLOCK), 0,
                                (hipStream_t)stream, b);
         }
     }, [&](auto dt) {
@@ -393,7 +410,7 @@ extern "C" int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, con
                                            q, scale}, stream);
 }
 
-extern "C" long long i2p_rms_norm_bwd_scratch(long long rows, int d) { return rows <= 0 || d <= 0 ? 0 : bwd_blocks(rows) * d * 4; }
+extern "C" long long i2p_rms_norm_bwd_scratch(long long rows, int d) { return rows <= 0 || d <= 0 ? 0 : bwd_blocks(rows, d, 256) * d * 4; }
 
 extern "C" int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, const void *s, long long lds, const void *gy, long long ldgy,
                                 const void *gs, long long ldgs, const void *w, const float *rstd, void *dx, void *dw, void *scratch, void *stream) {
@@ -402,12 +419,12 @@ extern "C" int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, co
     const BwdArgs a{rows, d, wdtype, (const char *)s, lds, (const char *)gy, ldgy, (const char *)gs, ldgs, w, rstd, (char *)dx,
                     dw ? (float *)scratch : nullptr};
     long long nblk = 0;
-    by_row(dtype, d, [&](auto dt, auto tpr, auto nv) {
+    by_row(dtype, d, [&](auto dt, auto tpr, auto nv, auto tiny) {
         constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
-        nblk = bwd_blocks((rows + RPB - 1) / RPB);
-        hipLaunchKernelGGL((rms_bwd_kernel<dt.value, tpr.value, nv.value>), dim3((unsigned)nblk), dim3(BLOCK), 0, (hipStream_t)stream, a);
+        nblk = bwd_blocks((rows + RPB - 1) / RPB, d, BLOCK);
+        hipLaunchKernelGGL((rms_bwd_kernel<dt.value, tpr.value, nv.value, tiny.value>), dim3((unsigned)nblk), dim3(BLOCK), 0, (hipStream_t)stream, a);
     }, [&](auto dt) {
-        nblk = bwd_blocks(rows);
+        nblk = bwd_blocks(rows, d, LT);
         hipLaunchKernelGGL((rms_bwd_long_kernel<dt.value>), dim3((unsigned)nblk), dim3(LT), 0, (hipStream_t)stream, a);
     });
     if (dw)

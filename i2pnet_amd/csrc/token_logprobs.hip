@@ -32,8 +32,30 @@ __device__ __forceinline__ float score_of(skey k) { return value_of((unsigned)(k
 __device__ __forceinline__ int64_t col_of(skey k) { return (int64_t)(0xffffffffu - (unsigned)k); }
 
 __device__ __forceinline__ float shift_of(float m) { return m == -__builtin_inff() ? 0.f : m; }
-// z e^z with 0 in the limit z -> -inf (e^-200 is 0)
-__device__ __forceinline__ float z_exp(float z, float e, float acc) { return __builtin_fmaf(fmaxf(z, -200.f), e, acc); }
+
+// The sums S = sum 2^y and U = sum y 2^y are formed with y = x log2(e) - c log2(e) in one multiply-add and one exponential per score.  The
+// rounding of c log2(e) shifts every y by the same `off`; it is known exactly and taken out of the sums afterwards.  Beyond FAR, where that
+// shift would grow, y = (x - c) log2(e) takes one operation more.
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f, FAR = 65536.f;
+struct Shift {
+    float c, c2, off;
+    bool far;
+    __device__ __forceinline__ explicit Shift(float m) : c(m), far(!(fabsf(m) < FAR)) {
+        c2 = c * LOG2E;
+        off = far ? 0.f : __builtin_fmaf(c, LOG2E, -c2);
+    }
+    template <bool FARAWAY> __device__ __forceinline__ void add(float x, float &S, float &U) const {
+        const float y = FARAWAY ? (x - c) * LOG2E : __builtin_fmaf(x, LOG2E, -c2), e = __builtin_amdgcn_exp2f(y);
+        S += e;
+        U = __builtin_fmaf(fmaxf(y, -300.f), e, U);             // (2^-300 is 0, and so is y 2^y in the limit)
+    }
+    // S and U = sum z e^z of z = x - c
+    __device__ __forceinline__ void finish(float &S, float &U) const {
+        U = LN2 * __builtin_fmaf(-off, S, U);
+        const float f = __builtin_amdgcn_exp2f(-off);
+        S *= f; U *= f;
+    }
+};
 
 struct FwdArgs {
     long long rows; int v; const char *x; long long ldx; const int64_t *ids; long long ignore; int top; float *logp, *entropy, *stat, *top_logp;
@@ -93,7 +115,7 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     const char *x = a.x + (row * a.ldx + lo) * i2p_esize(DT);
     if (id == a.ignore) { if (a.nsplit == 1) skip_row(a, row); return; }
     uint4 v[NV];
-    float most = -__builtin_inff();
+    float vmax[NV], most = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const Col<DT, TINY> c(j * T + t, n);
@@ -112,8 +134,10 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     for (int j = 0; j < NV; ++j) {
         float f[VE];
         unpack<DT>(v[j], f);
+        vmax[j] = f[0];
 #pragma unroll
-        for (int e = 0; e < VE; ++e) most = fmaxf(most, f[e]);
+        for (int e = 1; e < VE; ++e) vmax[j] = fmaxf(vmax[j], f[e]);
+        most = fmaxf(most, vmax[j]);
     }
     hold(v);
     // 64 groups of W lanes
@@ -136,13 +160,24 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
             if (__popcll(above) + __popcll(equal) == a.top - 1 && lane == 0) bound = gk;
         }
     }
+    const Shift sh(c);
     float S = 0.f, U = 0.f;
+    if (!sh.far) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float f[VE];
-        unpack<DT>(v[j], f);
+        for (int j = 0; j < NV; ++j) {
+            float f[VE];
+            unpack<DT>(v[j], f);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) { const float z = f[e] - c, ez = __expf(z); S += ez; U = z_exp(z, ez, U); }
+            for (int e = 0; e < VE; ++e) sh.template add<false>(f[e], S, U);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float f[VE];
+            unpack<DT>(v[j], f);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) sh.template add<true>(f[e], S, U);
+        }
     }
     hold(v);
     S = wave_sum(S); U = wave_sum(U);
@@ -153,6 +188,7 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
 #pragma unroll
         for (int w = 0; w < W; ++w) { S += sums[0][w]; U += sums[1][w]; }
     }
+    sh.finish(S, U);
     if (t == 0) {
         if (a.nsplit == 1) finish_row(a, row, id, xid, c, S, U);
         else a.part[row * a.nsplit + part] = make_float4(m, S, U, 0.f);
@@ -168,6 +204,7 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     if (plain && most >= least) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
+            if (!(vmax[j] >= least)) continue;
             const Col<DT, TINY> col(j * T + t, n);
             float f[VE];
             unpack<DT>(v[j], f);
@@ -316,11 +353,10 @@ template <class F> void by_type(int dtype, F f) {
 constexpr int WHOLE = 32768;                    // scores that 16 waves hold
 constexpr int SLICE = 8192;                     // 4 waves
 
-// how a row is cut: one block up to 32768 scores; longer rows in slices of at most that, or of at most 8192 where few rows would leave most
-// of the 256 CUs without one
+// how a row is cut: few rows of up to 32768 scores stay whole, which saves the second launch (the 256 CUs hold two blocks of 16 waves each);
+// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 88 us, slices 71 + 7; 8192 x 131072: 557, 522 + 13)
 inline void cut(long long rows, int v, int &nsplit, int &slice) {
-    nsplit = (v + WHOLE - 1) / WHOLE;
-    if (nsplit > 1 && rows * nsplit < 256) nsplit = (v + SLICE - 1) / SLICE;
+    nsplit = v <= WHOLE && rows <= 512 ? 1 : (v + SLICE - 1) / SLICE;
     slice = ((v + nsplit - 1) / nsplit + 7) & ~7;
     nsplit = (v + slice - 1) / slice;
 }
