@@ -153,6 +153,10 @@ HELPERS = {
 LONG_HELPERS = {"i2p_pair_lin_bwd_scratch", "i2p_pair_bias_bn_bwd_scratch", "i2p_gather_rows_grad_fx_scratch", "i2p_gemm_tn_scratch", "i2p_chain_sums_len", "i2p_chain_sync_words", "i2p_chain_bwd_slab",
                 "i2p_rms_norm_bwd_scratch", "i2p_token_logprobs_scratch", "i2p_grad_norm_scratch"}
 
+# what csrc/torch_rows.cpp calls, by address
+ROW_ENTRIES = ["i2p_rms_norm_fwd", "i2p_rms_norm_q8", "i2p_rms_norm_bwd", "i2p_rms_norm_bwd_scratch", "i2p_token_logprobs_fwd",
+               "i2p_token_logprobs_bwd", "i2p_token_logprobs_scratch", "i2p_clip_grad_norm", "i2p_grad_norm_scratch"]
+
 FLOAT_HELPERS = {"i2p_ktime_last_us"}
 
 _CT = {"l": C.c_longlong, "i": C.c_int, "f": C.c_float, "d": C.c_double, "p": C.c_void_p, "pp": C.c_void_p}

@@ -45,6 +45,24 @@ def load():
     return _lib
 
 
+_ROWS_PATH = Path(__file__).resolve().parent / "lib" / "torch_rows.so"
+
+
+def load_rows():
+    """the extension module of csrc/torch_rows.cpp, with the addresses of its entries in libi2p_ops.so.  No fallback, as above"""
+    import importlib.util
+
+    import torch  # noqa: F401  (the extension links against its libraries)
+    load()
+    if not _ROWS_PATH.exists():
+        raise I2POpsError(f"{_ROWS_PATH} not found: build it with `python -m i2pnet_amd.build`")
+    spec = importlib.util.spec_from_file_location("_torch_rows", _ROWS_PATH)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind({n: C.cast(getattr(_lib, n), C.c_void_p).value for n in _abi.ROW_ENTRIES if hasattr(_lib, n)})
+    return mod
+
+
 def helper(name, *args):
     """plain `int f(ints...)` helpers of the ABI (grid sizes of scratch buffers)"""
     load()

@@ -32,6 +32,8 @@ EXTRA_FLAGS = {"mlp_wreg.hip": ["-mllvm", "-pragma-unroll-threshold=1000000"],
                "image_first.hip": ["-fno-slp-vectorize"]}
 if os.environ.get("WREG_ABL"):      # diagnostic build of the ablation switches in mlp_wreg.hip
     EXTRA_FLAGS["mlp_wreg.hip"].append("-DWREG_ABL=" + os.environ["WREG_ABL"])
+# the torch side of the row operators: host code, compiled by g++ against torch's headers
+ROWS_SRC, ROWS_LIB = CSRC / "torch_rows.cpp", PKG / "lib" / "torch_rows.so"
 HEADERS = [CSRC / "common.h", PKG.parent / "include" / "i2p_ops.h"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
@@ -55,8 +57,19 @@ def _stale(target, deps):
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def _rows_command():
+    import sysconfig
+
+    import torch
+    t = Path(torch.__file__).resolve().parent
+    inc = [t / "include", t / "include" / "torch" / "csrc" / "api" / "include", "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wno-unknown-pragmas", "-D__HIP_PLATFORM_AMD__=1",
+             "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{i}" for i in inc] + [str(ROWS_SRC), f"-L{t / 'lib'}",
+            "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip", "-o", str(ROWS_LIB)])
+
+
 def needs_build():
-    return _stale(LIB, [CSRC / s for s in _sources()] + HEADERS + list(CSRC.glob("*.h")))
+    return _stale(ROWS_LIB, [ROWS_SRC] + HEADERS) or _stale(LIB, [CSRC / s for s in _sources()] + HEADERS + list(CSRC.glob("*.h")))
 
 
 def build(force=False, verbose=True):
@@ -80,6 +93,9 @@ def build(force=False, verbose=True):
         if verbose:
             print("[i2pnet_amd.build]", " ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, cwd=str(CSRC))
+
+    if force or _stale(ROWS_LIB, [ROWS_SRC] + HEADERS):
+        jobs.append(_rows_command())
 
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(run, jobs))

@@ -60,26 +60,6 @@ def Get_loss(out3, out4, qq_gt, t_gt, w_x, w_q, cfg):
 TokenLogprobs = namedtuple("TokenLogprobs", ["logp", "entropy", "top_logp", "top_ids"])
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, top, ignore_index):
-        logp, entropy, top_logp, top_ids, x2, ids, stat = ops.get_backend().token_logprobs_forward(logits, ids, top, ignore_index)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top_logp, top_ids)
-        ctx.save_for_backward(x2, ids, stat, entropy)
-        ctx.ignore_index, ctx.shape = ignore_index, logits.shape
-        return logp, entropy, top_logp, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logp, g_entropy, _g_top, _g_ids):
-        if g_logp is None and g_entropy is None:
-            return None, None, None, None
-        x2, ids, stat, entropy = ctx.saved_tensors
-        dx = ops.get_backend().token_logprobs_backward(x2, ids, ctx.ignore_index, stat, entropy, g_logp, g_entropy)
-        return dx.view(ctx.shape), None, None, None
-
-
 def token_logprobs(logits, ids, top=0, ignore_index=-100):
     """Log probabilities of the candidates `ids` [...] under softmax(logits [..., v]), with the entropy of every row and its `top` best
     alternatives -> TokenLogprobs(logp [...], entropy [...], top_logp [..., top], top_ids [..., top]), float32 and int64.  The matching loss of
@@ -90,4 +70,4 @@ def token_logprobs(logits, ids, top=0, ignore_index=-100):
     gradient 0.  Any other id outside [0, v) makes that row's logp and gradient NaN (ids are not read on the host).  A row without
     candidates (all -inf) has logp -inf, entropy 0 and gradient 0; a NaN or +inf makes the row's results NaN.
     top: 0 .. min(v, 32); equal scores are listed by index.  logp and entropy are differentiable in logits, once; the alternatives are not."""
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, ids, int(top), int(ignore_index)))
+    return TokenLogprobs(*ops.rows().token_logprobs(logits, ids, top, ignore_index))

@@ -682,28 +682,6 @@ def _unit_variance(x):
     return (x - torch.mean(x, -1, keepdim=True)) / torch.clip(torch.std(x, -1, keepdim=True), min=1e-12)
 
 
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        be = ops.get_backend()
-        y, s, rstd = be.rms_norm_forward(x, weight, residual, eps, want_rstd=any(ctx.needs_input_grad))
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(s, weight, rstd)
-        ctx.shape = x.shape
-        return y if residual is None else (y, s)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, gs=None):
-        s, weight, rstd = ctx.saved_tensors
-        need_dw = weight is not None and ctx.needs_input_grad[2]
-        if gy is None:                      # only the stream is used further on (or nothing is)
-            return gs, gs if ctx.needs_input_grad[1] else None, None, None
-        like = s.view(ctx.shape)
-        dx, dw = ops.get_backend().rms_norm_backward(like, weight, rstd, gy, gs, need_dw)
-        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
-
-
 def rms_norm(x, weight=None, residual=None, eps=1e-6):
     """y = s * weight / sqrt(mean(s^2, -1) + eps) over the last axis, of s = x, or with `residual` of the stream s = x + residual as it is
     stored (rounded to x's type); returns y, or (y, s).  One launch forward, two backward (csrc/rms_norm.hip): unlike the batch-statistics
@@ -711,16 +689,15 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
 
     x, residual: [..., d] float32, bfloat16 or float16 of any d and row pitch (rows without unit column stride are copied first);
     weight: [d], float32 or x's type, None = ones.  Differentiable in x, residual and weight, once."""
-    return _RmsNorm.apply(x, residual, weight, float(eps))
+    r = ops.rows()
+    return r.rms_norm(x, weight, eps) if residual is None else r.rms_norm_residual(x, weight, residual, eps)
 
 
 def rms_norm_q8(x, weight=None, residual=None, eps=1e-6, group=0):
     """`rms_norm` whose output feeds an 8-bit product: -> (q float8_e4m3fn [..., d], scale float32 [..., ceil(d / group)]) and, with `residual`,
     the stream s as a third; q * scale is the norm's output.  One scale per row (group = 0) or per `group` columns (a power of two,
     32 .. 512).  A group of zeros has scale 1, one with a NaN or inf scale inf.  For inference: refused where a gradient would be needed."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, residual)):
-        raise RuntimeError("rms_norm_q8 has no gradient: call it under torch.no_grad() or on detached tensors")
-    q, scale, s = ops.get_backend().rms_norm_q8(x, weight, residual, float(eps), int(group))
+    q, scale, s = ops.rows().rms_norm_q8(x, weight, residual, eps, group)
     return (q, scale) if residual is None else (q, scale, s)
 
 

@@ -8,7 +8,6 @@ surfaces of the reference (`fused_conv_g.cpp:15-67`, `pointnet2/src/pointnet2_ap
 `set_backend()` exists so that tests and bench.py's cpu_baseline leg can run the host logic
 against the CPU oracle; nothing in this package ever installs a non-HIP backend.
 """
-import array
 import ctypes as C
 
 import contextlib
@@ -21,7 +20,6 @@ from . import _abi, _lib
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
 _BF16 = torch.bfloat16
 BN_REPLICAS = 32          # I2P_BN_REPLICAS in include/i2p_ops.h
-_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}       # I2P_F32, I2P_BF16, I2P_F16
 MAX_TOP = 32              # I2P_MAX_TOP
 MAX_CANDIDATES = 1 << 21  # I2P_MAX_CANDIDATES
 
@@ -1403,140 +1401,31 @@ class CBackend:
                    self._p(d_pix, _F32, "d_pix"), stream=self._stream())
         return d_pts, d_pix
 
-    # ---- row operators (csrc/rms_norm.hip, token_logprobs.hip, grad_norm.hip; device library only) ---------------
-    def _row_arg(self, t, like, what):
-        """t [..., d] -> (t as [rows, d] with unit column stride, row pitch): a copy only where the rows are not laid out so.  `like`: the
-        tensor whose type, device and shape it has to share, or None"""
-        if not isinstance(t, torch.Tensor) or t.device.type != self.device_type:
-            raise RuntimeError(f"{what} must be a {self.device_type} tensor (got {getattr(t, 'device', type(t))})")
-        if t.dtype not in _ROW_TYPES:
-            raise RuntimeError(f"{what} must be float32, bfloat16 or float16 (got {t.dtype})")
-        if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-            raise RuntimeError(f"{what} must be {like.dtype} {tuple(like.shape)} on {like.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
-        if t.dim() == 0 or t.shape[-1] == 0:
-            raise RuntimeError(f"{what} must have rows of at least one element (got {tuple(t.shape)})")
-        d = t.shape[-1]
-        t2 = t if t.dim() == 2 else t.reshape(-1, d)
-        rows = t2.shape[0]
-        if (d > 1 and t2.stride(1) != 1) or (rows > 1 and t2.stride(0) < d):
-            t2 = t2.contiguous()
-        return t2, (t2.stride(0) if rows > 1 else d)
-
-    def _call_on(self, device, name, *args):
-        """the call on `device`'s current stream, whichever device is current"""
-        if device.index == torch.cuda.current_device():
-            self._call(name, *args, stream=torch.cuda.current_stream().cuda_stream)
-        else:
-            with torch.cuda.device(device):
-                self._call(name, *args, stream=torch.cuda.current_stream().cuda_stream)
-
-    @staticmethod
-    def _ptr(t):
-        return None if t is None else t.data_ptr()
-
-    def _rms_args(self, x, residual, weight):
-        x2, ldx = self._row_arg(x, None, "x")
-        r2, ldr = self._row_arg(residual, x, "residual") if residual is not None else (None, 0)
-        d = x2.shape[1]
-        if d > 0x7fffffff:
-            raise RuntimeError(f"x: rows of {d} elements are too long")
-        if weight is not None and (weight.device != x.device or weight.shape != (d,) or weight.dtype not in (_F32, x.dtype) or not weight.is_contiguous()):
-            raise RuntimeError(f"weight must be a contiguous float32 or {x.dtype} [{d}] on {x.device} (got {weight.dtype} {tuple(weight.shape)} on {weight.device})")
-        return x2, ldx, r2, ldr, d, _ROW_TYPES[x.dtype], _ROW_TYPES[weight.dtype] if weight is not None else 0
-
+    # ---- row operators (csrc/rms_norm.hip, token_logprobs.hip, grad_norm.hip through csrc/torch_rows.cpp; device library only) --------
     def rms_norm_forward(self, x, weight, residual, eps, want_rstd=True):
         """x, residual [..., d] -> (y, the stream s = x + residual (x as rows where residual is None), rstd [rows] or None)"""
-        x2, ldx, r2, ldr, d, dt, wt = self._rms_args(x, residual, weight)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r2 is not None else None
-        rstd = torch.empty(x2.shape[0], dtype=_F32, device=x.device) if want_rstd else None
-        self._call_on(x.device, "i2p_rms_norm_fwd", x2.shape[0], d, dt, wt, x2.data_ptr(), ldx, self._ptr(r2), ldr, self._ptr(weight), eps,
-                      self._ptr(s), y.data_ptr(), self._ptr(rstd))
-        return y, (x2 if s is None else s), rstd
+        return rows().rms_norm_forward(x, weight, residual, eps, want_rstd)
 
     def rms_norm_q8(self, x, weight, residual, eps, group):
         """-> (q float8_e4m3fn like x, scale f32 [..., groups], s or None)"""
-        x2, ldx, r2, ldr, d, dt, wt = self._rms_args(x, residual, weight)
-        if group != 0 and (group < 32 or group > 512 or group & (group - 1)):
-            raise ValueError(f"rms_norm_q8: group must be 0 (the whole row) or a power of two from 32 to 512 (got {group})")
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(*x.shape[:-1], -(-d // group) if group else 1, dtype=_F32, device=x.device)
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r2 is not None else None
-        self._call_on(x.device, "i2p_rms_norm_q8", x2.shape[0], d, dt, wt, x2.data_ptr(), ldx, self._ptr(r2), ldr, self._ptr(weight), eps, group,
-                      self._ptr(s), q.data_ptr(), scale.data_ptr())
-        return q, scale, s
+        return rows().rms_norm_q8(x, weight, residual, eps, group)
 
     def rms_norm_backward(self, s, weight, rstd, gy, gs, need_dw):
-        """s, gy, gs [..., d] (gs None: no gradient reaches the stream) -> (dx like s, dw like weight or None)"""
-        s2, lds = self._row_arg(s, None, "s")
-        gy2, ldg = self._row_arg(gy, s, "gy")
-        gs2, ldgs = self._row_arg(gs, s, "gs") if gs is not None else (None, 0)
-        rows, d = s2.shape
-        dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
-        if rows == 0:
-            return dx, torch.zeros_like(weight) if need_dw else None
-        dw = torch.empty_like(weight) if need_dw else None
-        scratch = torch.empty(_lib.helper("i2p_rms_norm_bwd_scratch", rows, d), dtype=torch.uint8, device=s.device) if need_dw else None
-        self._call_on(s.device, "i2p_rms_norm_bwd", rows, d, _ROW_TYPES[s.dtype], _ROW_TYPES[weight.dtype] if weight is not None else 0, s2.data_ptr(),
-                      lds, gy2.data_ptr(), ldg, self._ptr(gs2), ldgs, self._ptr(weight), rstd.data_ptr(), dx.data_ptr(), self._ptr(dw),
-                      self._ptr(scratch))
-        return dx, dw
+        """s, gy, gs [..., d] (gs None: no gradient reaches the stream) -> (dx like gy, dw like weight or None)"""
+        return rows().rms_norm_backward(s, weight, rstd, gy, gs, need_dw)
 
     def token_logprobs_forward(self, logits, ids, top, ignore_index):
         """logits [..., v], ids i64 [...] -> (logp [...], entropy [...], top_logp [..., top], top_ids [..., top], logits as rows, ids, stat)"""
-        x2, ldx = self._row_arg(logits, None, "logits")
-        rows, v = x2.shape
-        if not isinstance(ids, torch.Tensor) or ids.dtype != _I64 or ids.device != logits.device or ids.shape != logits.shape[:-1]:
-            raise RuntimeError(f"ids must be int64 {tuple(logits.shape[:-1])} on {logits.device} "
-                               f"(got {getattr(ids, 'dtype', type(ids))} {tuple(getattr(ids, 'shape', ()))} on {getattr(ids, 'device', None)})")
-        if not 0 <= top <= min(v, MAX_TOP):
-            raise ValueError(f"token_logprobs: top must be between 0 and {min(v, MAX_TOP)} (got {top})")
-        if v > MAX_CANDIDATES:
-            raise ValueError(f"token_logprobs: rows of at most {MAX_CANDIDATES} candidates (got {v})")
-        ids = ids.contiguous()
-        dev, dt = logits.device, _ROW_TYPES[logits.dtype]
-        logp, entropy = torch.empty(ids.shape, dtype=_F32, device=dev), torch.empty(ids.shape, dtype=_F32, device=dev)
-        stat = torch.empty(rows, 2, dtype=_F32, device=dev)
-        top_logp = torch.empty(*ids.shape, top, dtype=_F32, device=dev)
-        top_ids = torch.empty(*ids.shape, top, dtype=_I64, device=dev)
-        nbytes = _lib.helper("i2p_token_logprobs_scratch", rows, v, dt, top)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        self._call_on(dev, "i2p_token_logprobs_fwd", rows, v, dt, x2.data_ptr(), ldx, ids.data_ptr(), ignore_index, top, logp.data_ptr(),
-                      entropy.data_ptr(), stat.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(), self._ptr(scratch))
-        return logp, entropy, top_logp, top_ids, x2, ids, stat
+        return rows().token_logprobs_forward(logits, ids, top, ignore_index)
 
     def token_logprobs_backward(self, x2, ids, ignore_index, stat, entropy, g_logp, g_entropy):
-        """-> dlogits [rows, v]"""
-        rows, v = x2.shape
-        dx = torch.empty(rows, v, dtype=x2.dtype, device=x2.device)
-        gl, gh = (g.contiguous() if g is not None else None for g in (g_logp, g_entropy))
-        self._call_on(x2.device, "i2p_token_logprobs_bwd", rows, v, _ROW_TYPES[x2.dtype], x2.data_ptr(), x2.stride(0) if rows > 1 else v,
-                      ids.data_ptr(), ignore_index, stat.data_ptr(), entropy.data_ptr(), self._ptr(gl), self._ptr(gh), dx.data_ptr())
-        return dx
+        """-> dlogits like x2"""
+        return rows().token_logprobs_backward(x2, ids, ignore_index, stat, entropy, g_logp, g_entropy)
 
     def clip_grad_norm(self, grads, kind, max_norm, out=None):
         """Norm of a list of dense gradients (kind 0: 2-norm, 1: largest magnitude) -> f32 0-d; max_norm None: nothing is clipped, else in
         place or into the flat fp32 buffer `out` (include/i2p_ops.h i2p_clip_grad_norm)"""
-        device = grads[0].device
-        types = [_ROW_TYPES.get(g.dtype, -1) for g in grads]
-        if min(types) < 0:
-            raise RuntimeError("gradients must be float32, bfloat16 or float16")
-        if device.type != self.device_type or any(g.device != device for g in grads):
-            raise RuntimeError(f"gradients must be {self.device_type} tensors on one device")
-        if not all(g.is_contiguous() or g.is_contiguous(memory_format=torch.channels_last) for g in grads):
-            raise RuntimeError("gradients must be dense (contiguous or channels_last)")
-        n = len(grads)
-        ptrs, sizes = array.array("Q", [g.data_ptr() for g in grads]), array.array("q", [g.numel() for g in grads])
-        kinds = array.array("i", types)
-        if out is not None and (not isinstance(out, torch.Tensor) or out.device != device or out.dtype != _F32 or out.dim() != 1
-                                or not out.is_contiguous() or out.numel() != sum(sizes)):
-            raise RuntimeError(f"out must be a contiguous float32 [{sum(sizes)}] on {device}")
-        sizes_p = sizes.buffer_info()[0]
-        scratch = torch.empty(_lib.helper("i2p_grad_norm_scratch", n, sizes_p), dtype=torch.uint8, device=device)
-        total = torch.empty((), dtype=_F32, device=device)
-        self._call_on(device, "i2p_clip_grad_norm", n, ptrs.buffer_info()[0], sizes_p, kinds.buffer_info()[0], kind, max_norm is not None,
-                      0.0 if max_norm is None else max_norm, self._ptr(out), scratch.data_ptr(), total.data_ptr())
-        return total
+        return rows().clip_grad_norm(grads, kind, max_norm, out)
 
     def bn_finalize(self, rows, sums, gamma, beta, eps):
         """-> (coef [3,c] = mean, invstd*gamma, beta ; mean_invstd [2c])"""
@@ -1551,6 +1440,15 @@ class CBackend:
 
 _hip = None
 _active = None
+_rows = None
+
+
+def rows():
+    """The torch side of the row operators (csrc/torch_rows.cpp: checks, outputs, autograd nodes), bound to the loaded libi2p_ops.so"""
+    global _rows
+    if _rows is None:
+        _rows = _lib.load_rows()
+    return _rows
 
 
 def hip_backend():

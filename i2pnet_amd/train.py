@@ -142,15 +142,7 @@ class FlatAdam:
 
 def _grad_list(parameters):
     """the gradients meant by a list of parameters (those that have one) and plain gradient tensors"""
-    grads = []
-    for t in [parameters] if isinstance(parameters, torch.Tensor) else parameters:
-        if type(t) is torch.Tensor and not t.requires_grad:
-            grads.append(t)
-        elif not isinstance(t, torch.Tensor) or not t.is_leaf:
-            raise RuntimeError(f"parameters (leaves) or gradient tensors are wanted (got {type(t).__name__})")
-        elif t.grad is not None:
-            grads.append(t.grad)
-    return grads
+    return ops.rows().grad_list(parameters)
 
 
 def _norm_kind(norm_type):
@@ -161,17 +153,13 @@ def _norm_kind(norm_type):
     raise ValueError(f"norm_type must be 2 or inf (got {norm_type})")
 
 
-@torch.no_grad()
 def grad_norm(parameters, norm_type=2.0):
     """Global norm (2, or inf: the largest magnitude) of the gradients of `parameters` -> float32 0-d tensor on their device; the host does
     not wait.  `parameters`: parameters, whose .grad is meant (those without one are skipped), or gradient tensors themselves."""
-    grads, kind = _grad_list(parameters), _norm_kind(norm_type)
-    if not grads:
-        return torch.zeros((), device="cuda")
-    return ops.get_backend().clip_grad_norm(grads, kind, None)
+    total = ops.rows().clip_parameters(parameters, _norm_kind(norm_type), None, None)
+    return torch.zeros((), device="cuda") if total is None else total
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
     """Clips the gradients of `parameters` to a global norm of at most `max_norm` (times min(1, max_norm / (norm + 1e-6))) and returns the norm
     before it, without waiting for the device: what `FlatAdam.fused_clip_step` does for the trainer's flat buffer, for any list of
@@ -181,18 +169,19 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     parameters: see `grad_norm`; dense float32, bfloat16 and float16 tensors of one device, mixed; tensors that share memory are refused
     in place.  A NaN or inf norm makes every gradient NaN or 0, as torch's function does; error_if_nonfinite raises instead (it waits for
     the device) and leaves them as they are."""
-    grads, kind, max_norm = _grad_list(parameters), _norm_kind(norm_type), float(max_norm)
+    kind, max_norm = _norm_kind(norm_type), float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative (got {max_norm})")
-    if not grads:
+    if error_if_nonfinite:
+        parameters = _grad_list(parameters)
+        total = ops.rows().clip_parameters(parameters, kind, None, None)
+        if total is not None and not bool(torch.isfinite(total)):
+            raise RuntimeError("the global norm of the gradients is not finite: they were not clipped")
+    total = ops.rows().clip_parameters(parameters, kind, max_norm, out)
+    if total is None:
         if out is not None and out.numel():
             raise RuntimeError("out must be empty: there is no gradient")
         return torch.zeros((), device="cuda")
-    be = ops.get_backend()
-    if error_if_nonfinite and not bool(torch.isfinite(be.clip_grad_norm(grads, kind, None))):
-        raise RuntimeError("the global norm of the gradients is not finite: they were not clipped")
-    total = be.clip_grad_norm(grads, kind, max_norm, out)
-    torch.autograd.graph.increment_version(grads if out is None else out)
     return total
 
 

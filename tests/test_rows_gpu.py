@@ -233,8 +233,9 @@ def test_more_rows_than_one_launch_takes():
 # ---- log probabilities -----------------------------------------------------------------------------------------------------------
 def logp64(x, ids, top, gl=None, gh=None):
     a = x.double()
-    L = torch.logsumexp(a, -1, keepdim=True)
-    lp = a - L
+    m = a.amax(-1, keepdim=True)
+    z = a - torch.where(m.isfinite(), m, torch.zeros_like(m))             # (3e38 + 8 is 3e38 in 64 bits too)
+    lp = z - torch.logsumexp(z, -1, keepdim=True)
     p = lp.exp()
     plogp = torch.special.xlogy(p, p)
     H = -plogp.sum(-1, keepdim=True)
@@ -643,3 +644,50 @@ def test_the_rows_behind_a_batch_stay_as_they_are():
     g = [torch.ones(300, device=DEV, dtype=torch.bfloat16), torch.ones(77, device=DEV)]
     train.clip_grad_norm_(g, 1.0, out=buf[100:477])
     assert buf[:100].eq(9).all() and buf[477:].eq(9).all() and not buf[100:477].eq(9).any()
+
+
+@pytest.mark.parametrize("far", [1e5, -1e5, 3e38, -3e38, 1e30])
+def test_token_logprobs_maximum_far_from_zero(far):
+    """a maximum beyond the range where its logarithm's rounding is carried along, up to the type's largest values"""
+    v = 3000
+    x = far + (rnd(4, v, seed=2) * (4.0 if abs(far) < 1e6 else 1e-3 * abs(far)))
+    x[1] = far                                              # uniform
+    x[2, 5:] = torch.finfo(torch.float32).min
+    x[3, 5:] = -math.inf
+    ids = torch.tensor([0, 1, 2, 3])
+    gl, gh = torch.ones(4), 0.5 * torch.ones(4)
+    lp, H, tl, ti, dx, mag = logp64(x, ids, 4, gl, gh)
+    leaf = x.to(DEV).requires_grad_(True)
+    o = loss.token_logprobs(leaf, ids.to(DEV), top=4)
+    # z of the given candidate is one subtraction off: U of the larger operand, at most 2 U |far| where that is below 1e6
+    near = 2 * U * abs(far) if abs(far) < 1e6 else 0.0
+    lp, tl = (t.masked_fill(t < -3.4e38, -math.inf) for t in (lp, tl))
+    big = lambda t: torch.where(t < -1e30, t.abs() * 4 * U, logp_tol(v, t.clamp_min(-1e37), 16) + near)
+    within(o.logp, lp, big(lp.clamp_min(-3.5e38)), "logp")
+    within(o.top_logp, tl, big(tl.clamp_min(-3.5e38)), "top_logp")
+    assert torch.equal(o.top_ids.cpu(), ti)
+    within(o.entropy, H, (chain(v) + 64) * U * 33 * torch.ones_like(H) + 32 * near, "entropy")
+    (d,) = torch.autograd.grad([o.logp, o.entropy], leaf, [gl.to(DEV), gh.to(DEV)])
+    within(d, dx, U * dx.abs() + (8 * chain(v) + 2000) * U * mag + 64 * near * mag + 1e-36, "dlogits")
+
+
+def test_double_backward_is_refused():
+    for f in (lambda a: modules.rms_norm(a, None), lambda a: loss.token_logprobs(a, torch.zeros(3, dtype=torch.long, device=DEV)).logp):
+        a = rnd(3, 9, seed=1).to(DEV).requires_grad_(True)
+        (g,) = torch.autograd.grad(f(a).sum(), a, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.square().sum().backward()
+
+
+def test_what_a_backward_pass_needs_may_not_be_changed():
+    a, w = rnd(3, 9, seed=1).to(DEV).requires_grad_(True), rnd(9, seed=2).to(DEV).requires_grad_(True)
+    y, s = modules.rms_norm(a, w, residual=a)
+    with torch.no_grad():
+        s.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    b = torch.zeros(9, device=DEV, requires_grad=True)
+    y = (b * b).sum()
+    train.clip_grad_norm_([b.detach()], 1.0)                # clipping counts as a change too
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
