@@ -8,33 +8,45 @@
 #include "rows_common.h"
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 namespace {
 
-constexpr int T = 256, CHUNK = 16384;
-constexpr int CAP = 180;                        // 20 bytes each: the table stays below the 4 KB of a kernel's arguments
+constexpr int T = 256;
 constexpr long long PART = 1ll << 30;           // a longer tensor is listed in parts of this many elements
 
-struct Table {
+// The tensors of a launch, by value (below the 4 KB of a kernel's arguments).  Where each starts in the flat output is listed only for a
+// launch that writes there, so that in place and for the norm one launch takes 320 tensors
+template <bool OUT> struct Table {
+    static constexpr int CAP = OUT ? 192 : 320;
     unsigned long long ptr[CAP];                // address | (elements of the last chunk - 1) << 48
+    unsigned long long off[OUT ? CAP : 1];
     unsigned first[CAP];                        // first chunk | dtype << 30
-    unsigned long long off[CAP];                // where it starts in the flat output
     unsigned n, chunks;
+    int chunk;                                  // elements of a chunk
 };
 
 struct Piece { unsigned long long p; int dtype; unsigned count; unsigned long long off; };
 
-// the piece of the table that chunk `c` of this launch covers
-__device__ __forceinline__ Piece piece_of(const Table &t, unsigned c) {
-    unsigned lo = 0, hi = t.n;                  // first[lo] <= c < first[hi]
-    while (hi - lo > 1) { const unsigned mid = (lo + hi) >> 1; if ((t.first[mid] & 0x3fffffffu) <= c) lo = mid; else hi = mid; }
-    const unsigned f = t.first[lo], k = c - (f & 0x3fffffffu), end = lo + 1 < t.n ? (t.first[lo + 1] & 0x3fffffffu) : t.chunks;
-    const unsigned long long p = t.ptr[lo];
+// The piece of the table that chunk `c` of this launch covers.  Every wave finds it by itself: each lane counts the tensors of its share that
+// start at or before the chunk (independent loads: a binary search is eight dependent ones, 2 .. 3 us of a 5 us kernel)
+template <bool OUT> __device__ __forceinline__ Piece piece_of(const Table<OUT> &t, unsigned c) {
+    constexpr int PER = Table<OUT>::CAP / 64;
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const unsigned i = k * 64 + lane;
+        before += __popcll(__ballot(i < t.n && (t.first[i] & 0x3fffffffu) <= c));
+    }
+    const int at = __builtin_amdgcn_readfirstlane(before) - 1;
+    const unsigned f = t.first[at], k = c - (f & 0x3fffffffu), end = at + 1 < (int)t.n ? (t.first[at + 1] & 0x3fffffffu) : t.chunks;
+    const unsigned long long p = t.ptr[at];
     Piece r;
     r.dtype = (int)(f >> 30);
-    r.p = (p & 0xffffffffffffull) + (unsigned long long)k * CHUNK * i2p_esize(r.dtype);
-    r.count = c + 1 == end ? (unsigned)(p >> 48) + 1u : (unsigned)CHUNK;
-    r.off = t.off[lo] + (unsigned long long)k * CHUNK;
+    r.p = (p & 0xffffffffffffull) + (unsigned long long)k * t.chunk * i2p_esize(r.dtype);
+    r.count = c + 1 == end ? (unsigned)(p >> 48) + 1u : (unsigned)t.chunk;
+    r.off = OUT ? t.off[at] + (unsigned long long)k * t.chunk : 0ull;
     return r;
 }
 
@@ -80,7 +92,7 @@ template <int DT, bool MAX> __device__ __forceinline__ double norm_piece(const P
     return acc;
 }
 
-template <bool MAX> __global__ __launch_bounds__(T) void grad_norm_kernel(Table t, double *__restrict__ partials) {
+template <bool MAX> __global__ __launch_bounds__(T) void grad_norm_kernel(Table<false> t, double *__restrict__ partials) {
     __shared__ double red[T / 64];
     const Piece p = piece_of(t, blockIdx.x);
     const double acc = p.dtype == I2P_F32 ? norm_piece<I2P_F32, MAX>(p) : p.dtype == I2P_BF16 ? norm_piece<I2P_BF16, MAX>(p) : norm_piece<I2P_F16, MAX>(p);
@@ -88,61 +100,92 @@ template <bool MAX> __global__ __launch_bounds__(T) void grad_norm_kernel(Table 
     if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-template <bool MAX> __global__ __launch_bounds__(1024) void grad_total_kernel(unsigned n, const double *__restrict__ partials, float *__restrict__ total) {
-    __shared__ double red[16];
+// the partial norms in a fixed order, the same on every block of as many threads
+template <bool MAX, int THREADS> __device__ __forceinline__ float total_of(unsigned n, const double *__restrict__ partials, double *red) {
     double acc = 0.0;
-    for (unsigned i = threadIdx.x; i < n; i += 1024) acc = MAX ? nan_max(acc, partials[i]) : acc + partials[i];
+    for (unsigned i0 = threadIdx.x; i0 < n; i0 += 8 * THREADS) {      // eight loads in flight
+        double p[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) p[u] = i0 + u * THREADS < n ? partials[i0 + u * THREADS] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc = MAX ? nan_max(acc, p[u]) : acc + p[u];
+    }
     const double s = block_sum<MAX>(acc, red);
-    if (threadIdx.x == 0) total[0] = (float)(MAX ? s : sqrt(s));
+    return (float)(MAX ? s : sqrt(s));
 }
 
-template <int DT> __device__ __forceinline__ void clip_piece(const Piece &p, float c, float *out) {
+template <bool MAX> __global__ __launch_bounds__(1024) void grad_total_kernel(unsigned n, const double *__restrict__ partials, float *__restrict__ total) {
+    __shared__ double red[16];
+    const float t = total_of<MAX, 1024>(n, partials, red);
+    if (threadIdx.x == 0) total[0] = t;
+}
+
+template <int DT, bool OUT> __device__ __forceinline__ void clip_piece(const Piece &p, float c, float *out) {
     constexpr int VE = i2p_vec(DT);
     for_vectors<DT>(p, [&](const float (&g)[VE], unsigned i) {
         float h[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) h[e] = g[e] * c;
-        if (out) __builtin_memcpy(out + p.off + i, h, 4 * VE);
+        if (OUT) __builtin_memcpy(out + p.off + i, h, 4 * VE);
         else { const uint4 u = pack<DT>(h); __builtin_memcpy((char *)p.p + (size_t)i * i2p_esize(DT), &u, 16); }
     });
     const unsigned rest = p.count / VE * VE + threadIdx.x;
     if (rest < p.count) {
         const float g = ld1<DT>((const void *)p.p, rest) * c;
-        if (out) out[p.off + rest] = g;
+        if (OUT) out[p.off + rest] = g;
         else st1<DT>((void *)p.p, rest, g);
     }
 }
 
-__global__ __launch_bounds__(T) void grad_clip_kernel(Table t, float max_norm, const float *__restrict__ total, float *out) {
-    const float r = max_norm / (total[0] + 1e-6f), c = r > 1.f ? 1.f : r;                   // (NaN stays)
-    if (c == 1.f && !out) return;                                                            // within the limit: the gradients stay as they are
+// OUT: into the flat buffer.  SUM 0: the total is there; 1, 2: every block forms it (2-norm, maximum) from the partial norms
+template <bool OUT, int SUM>
+__global__ __launch_bounds__(T) void grad_clip_kernel(Table<OUT> t, float max_norm, unsigned n, const double *__restrict__ partials, float *total, float *out) {
+    __shared__ double red[T / 64];
+    float norm;
+    if constexpr (SUM != 0) {
+        norm = total_of<SUM == 2, T>(n, partials, red);
+        if (total && blockIdx.x == 0 && threadIdx.x == 0) total[0] = norm;
+    } else norm = total[0];
+    const float r = max_norm / (norm + 1e-6f), c = r > 1.f ? 1.f : r;                       // (NaN stays)
+    if (c == 1.f && !OUT) return;                                                            // within the limit: the gradients stay as they are
     const Piece p = piece_of(t, blockIdx.x);
-    if (p.dtype == I2P_F32) clip_piece<I2P_F32>(p, c, out);
-    else if (p.dtype == I2P_BF16) clip_piece<I2P_BF16>(p, c, out);
-    else clip_piece<I2P_F16>(p, c, out);
+    if (p.dtype == I2P_F32) clip_piece<I2P_F32, OUT>(p, c, out);
+    else if (p.dtype == I2P_BF16) clip_piece<I2P_BF16, OUT>(p, c, out);
+    else clip_piece<I2P_F16, OUT>(p, c, out);
 }
 
-inline long long chunks_of(long long numel) { return (numel + CHUNK - 1) / CHUNK; }
+inline long long chunks_of(long long numel, int chunk) { return (numel + chunk - 1) / chunk; }
 
-// Walks the list in tables of at most CAP pieces and calls launch(table) for each
-template <class F> void for_tables(int n, const void *const *grads, const long long *numel, const int *dtype, F launch) {
-    Table t;
+// A chunk is what a block reads (at most 65536 elements: 16 bits of `ptr` tell the last one's length): 4096 elements, one batch of loads a
+// thread, while there are few; else 16384 (300 M elements: 531 us in all, 577 with 65536)
+inline int chunk_for(int n, const long long *numel) {
+    long long total = 0;
+    for (int i = 0; i < n; ++i) total += numel[i];
+    return total <= (4ll << 20) ? 4096 : 16384;
+}
+
+// Walks the list in tables and calls launch(table) for each
+template <bool OUT, class F> void for_tables(int n, const void *const *grads, const long long *numel, const int *dtype, F launch) {
+    Table<OUT> t;
     t.n = t.chunks = 0;
+    t.chunk = chunk_for(n, numel);
     unsigned long long off = 0;
     for (int i = 0; i < n; ++i)
         for (long long done = 0; done < numel[i]; done += PART) {
             const long long k = std::min(PART, numel[i] - done);
-            if (t.n == CAP || t.chunks + chunks_of(k) > (1 << 22)) { launch(t); t.n = t.chunks = 0; }
-            const unsigned long long last = (unsigned long long)((k - 1) % CHUNK);
+            if (t.n == Table<OUT>::CAP || t.chunks + chunks_of(k, t.chunk) > (1 << 22)) { launch(t); t.n = t.chunks = 0; }
+            const unsigned long long last = (unsigned long long)((k - 1) % t.chunk);
             t.ptr[t.n] = ((unsigned long long)grads[i] + (unsigned long long)done * i2p_esize(dtype[i])) | (last << 48);
             t.first[t.n] = t.chunks | ((unsigned)dtype[i] << 30);
-            t.off[t.n] = off;
+            if (OUT) t.off[t.n] = off;
             off += (unsigned long long)k;
             ++t.n;
-            t.chunks += (unsigned)chunks_of(k);
+            t.chunks += (unsigned)chunks_of(k, t.chunk);
         }
     if (t.n) launch(t);
 }
+
+constexpr unsigned FEW = 2048;                  // partial norms that every clipping block sums itself: cheaper than a launch of one block for it
 
 struct Range { unsigned long long lo, hi; };
 
@@ -171,7 +214,8 @@ int check(int n, const void *const *grads, const long long *numel, const int *dt
             if (r[i].lo < o.hi && o.lo < r[i].hi) { delete[] r; return I2P_ERR_OVERLAP; }
         k = 0;                                  // (only read: the same tensor may be listed twice)
     }
-    std::sort(r, r + k, [](const Range &a, const Range &b) { return a.lo < b.lo; });
+    const auto below = [](const Range &a, const Range &b) { return a.lo < b.lo; };
+    if (!std::is_sorted(r, r + k, below)) std::sort(r, r + k, below);
     int rc = 0;
     for (int i = 1; i < k; ++i)
         if (r[i].lo < r[i - 1].hi) rc = I2P_ERR_OVERLAP;
@@ -183,8 +227,11 @@ int check(int n, const void *const *grads, const long long *numel, const int *dt
 
 extern "C" long long i2p_grad_norm_scratch(int n, const long long *numel) {
     long long c = 0;
-    for (int i = 0; numel && i < n; ++i)
-        for (long long done = 0; done < numel[i]; done += PART) c += chunks_of(std::min(PART, numel[i] - done));
+    if (n > 0 && numel) {
+        const int chunk = chunk_for(n, numel);
+        for (int i = 0; i < n; ++i)
+            for (long long done = 0; done < numel[i]; done += PART) c += chunks_of(std::min(PART, numel[i] - done), chunk);
+    }
     return 8 * std::max(c, 1ll);
 }
 
@@ -196,16 +243,29 @@ extern "C" int i2p_clip_grad_norm(int n, const void *const *grads, const long lo
     hipStream_t st = (hipStream_t)stream;
     double *partials = (double *)scratch;
     unsigned done = 0;
-    for_tables(n, grads, numel, dtype, [&](const Table &t) {
+    for_tables<false>(n, grads, numel, dtype, [&](const Table<false> &t) {
         if (kind) hipLaunchKernelGGL((grad_norm_kernel<true>), dim3(t.chunks), dim3(T), 0, st, t, partials + done);
         else hipLaunchKernelGGL((grad_norm_kernel<false>), dim3(t.chunks), dim3(T), 0, st, t, partials + done);
         done += t.chunks;
     });
-    if (kind) hipLaunchKernelGGL((grad_total_kernel<true>), dim3(1), dim3(1024), 0, st, done, partials, total);
-    else hipLaunchKernelGGL((grad_total_kernel<false>), dim3(1), dim3(1024), 0, st, done, partials, total);
-    if (clip)
-        for_tables(n, grads, numel, dtype, [&](const Table &t) {
-            hipLaunchKernelGGL(grad_clip_kernel, dim3(t.chunks), dim3(T), 0, st, t, max_norm, total, out);
-        });
+    const bool few = clip && done && done <= FEW;
+    if (!few) {
+        if (kind) hipLaunchKernelGGL((grad_total_kernel<true>), dim3(1), dim3(1024), 0, st, done, partials, total);
+        else hipLaunchKernelGGL((grad_total_kernel<false>), dim3(1), dim3(1024), 0, st, done, partials, total);
+    }
+    if (clip) {
+        float *sum = total;                     // the first launch's first block writes the total
+        auto go = [&](auto with_out) {
+            constexpr bool OUT = decltype(with_out)::value;
+            for_tables<OUT>(n, grads, numel, dtype, [&](const Table<OUT> &t) {
+                if (!few) hipLaunchKernelGGL((grad_clip_kernel<OUT, 0>), dim3(t.chunks), dim3(T), 0, st, t, max_norm, done, partials, total, out);
+                else if (kind) hipLaunchKernelGGL((grad_clip_kernel<OUT, 2>), dim3(t.chunks), dim3(T), 0, st, t, max_norm, done, partials, sum, out);
+                else hipLaunchKernelGGL((grad_clip_kernel<OUT, 1>), dim3(t.chunks), dim3(T), 0, st, t, max_norm, done, partials, sum, out);
+                sum = nullptr;
+            });
+        };
+        if (out) go(std::true_type{});
+        else go(std::false_type{});
+    }
     I2P_RETURN_LAUNCH_STATUS();
 }

@@ -9,8 +9,8 @@
 // Forward: bound by the one read of the scores.  A row, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at
 // most 32 scores a thread), so that the true maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k best
 // in the workspace and a second launch joins them.
-// Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those is a value that at least k scores reach and that
-// few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow that list
+// Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those (to 16 bits) is a value that at least k scores reach
+// and that few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow that list
 // and are searched k times instead.
 #include "rows_common.h"
 
@@ -105,7 +105,7 @@ template <int DT, int W, int E>
 __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8) void logprobs_fwd_kernel(FwdArgs a) {
     constexpr int T = 64 * W, VE = i2p_vec(DT), NV = E / VE;
     constexpr bool TINY = T * E == 512;
-    __shared__ float gmax[64], sums[2][W], bound;
+    __shared__ float gmax[64], sums[2][W];
     __shared__ skey list[LIST], best[W];
     __shared__ int count;
     const long long row = blockIdx.x / (unsigned)a.nsplit;      // (one row's slices stay together)
@@ -151,14 +151,17 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
         g = gmax[lane];
     } else if (t == 0) count = 0;
     const float m = wave_max(g), c = shift_of(m);
-    if (a.top) {                                                // each wave ranks 64 / W of the groups
-#pragma unroll 4
-        for (int i = 0; i < 64 / W; ++i) {
-            const int k = __builtin_amdgcn_readfirstlane(wave) * (64 / W) + i;
-            const float gk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), k));
-            const skey above = __ballot(g > gk), equal = __ballot(g == gk) & ((1ull << k) - 1ull);
-            if (__popcll(above) + __popcll(equal) == a.top - 1 && lane == 0) bound = gk;
+    // the largest value, to 16 bits of its order, that at least `top` groups reach
+    float least = -__builtin_inff();
+    if (a.top) {
+        const unsigned o = order_of(g);
+        unsigned b = 0u;
+#pragma unroll
+        for (int k = 31; k >= 16; --k) {
+            const unsigned next = b | (1u << k);
+            if (__popcll(__ballot(o >= next)) >= a.top) b = next;
         }
+        if (b > 0x007fffffu) least = value_of(b);               // (below: the order of -inf)
     }
     const Shift sh(c);
     float S = 0.f, U = 0.f;
@@ -198,9 +201,9 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
         if (a.nsplit == 1) put_top(a, row, rank, key, c, S);
         else a.keys[(row * a.nsplit + part) * a.top + rank] = key;
     };
-    if constexpr (W == 1) __syncthreads();                      // (`bound`, `count`)
-    const float least = bound;
+    if constexpr (W == 1) __syncthreads();                      // (`count`)
     const bool plain = S == S;                                  // no NaN, no +inf
+    unsigned bits = 0u;                                         // which of the thread's scores reach the bound
     if (plain && most >= least) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -210,10 +213,21 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
             unpack<DT>(v[j], f);
 #pragma unroll
             for (int e = 0; e < VE; ++e)
-                if (f[e] >= least && col.counts(e, n)) {
-                    const int at = atomicAdd(&count, 1);
-                    if (at < LIST) list[at] = key_of(f[e], (unsigned)(lo + col.at + e));
-                }
+                if (f[e] >= least && (least > -__builtin_inff() || col.counts(e, n))) bits |= 1u << (j * VE + e);
+        }
+    }
+    for (;;) {                                                  // one of each lane a turn; its value is read again, from the caches
+        const skey has = __ballot(bits != 0u);
+        if (!has) break;
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&count, __popcll(has));
+        base = __builtin_amdgcn_readfirstlane(base);
+        if (base >= LIST) break;
+        if (bits) {
+            const int i = __ffs(bits) - 1, at = base + __popcll(has & ((1ull << lane) - 1ull));
+            bits &= bits - 1u;
+            const int col = Col<DT, TINY>(i / VE * T + t, n).at + i % VE;
+            if (at < LIST) list[at] = key_of(ld1<DT>(x, col), (unsigned)(lo + col));
         }
     }
     __syncthreads();
@@ -246,7 +260,8 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     }
 }
 
-// Joins the slices of a row.  The k-th largest of the slices' best keys bounds the row's k best from below; a slice's keys are in order
+// Joins the slices of a row, whose keys are in order.  Their q-th keys, q = top / slices rounded up, bound the row's best from below: where
+// top / q slices, rounded up, have a q-th key of at least b, `top` keys are at least b
 constexpr int JT = 256;                         // = most slices of a row
 __global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype) {
     __shared__ float sums[3][JT / 64];
@@ -258,7 +273,8 @@ __global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype)
     if (id == a.ignore) { skip_row(a, row); return; }
     const float4 p = t < a.nsplit ? a.part[row * a.nsplit + t] : make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
     const skey *keys = a.keys + (row * a.nsplit + t) * a.top;
-    const skey mine = a.top && t < a.nsplit ? keys[0] : 0ull;
+    const int q = a.top ? (a.top + a.nsplit - 1) / a.nsplit : 1, need = (a.top + q - 1) / q;
+    const skey mine = a.top && t < a.nsplit ? keys[q - 1] : 0ull;
     float xid = 0.f;
     if (t == 0 && id >= 0 && id < a.v) {
         const long long i = row * a.ldx + id;
@@ -277,7 +293,7 @@ __global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype)
     if (a.top && t < a.nsplit) {
         int rank = 0;
         for (int k = 0; k < a.nsplit; ++k) rank += head[k] > mine;
-        if (rank == a.top - 1) bound = mine;
+        if (rank == need - 1) bound = mine;
     }
     __syncthreads();
     S = U = 0.f;
@@ -285,8 +301,8 @@ __global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype)
     for (int w = 0; w < JT / 64; ++w) { S += sums[1][w]; U += sums[2][w]; }
     if (t == 0) finish_row(a, row, id, xid, c, S, U);
     if (!a.top) return;
-    if (t < a.nsplit && mine >= bound)
-        for (int k = 0; k < a.top; ++k) {                       // (at most `top` slices reach the bound, unless there are fewer slices)
+    if (t < a.nsplit)
+        for (int k = 0; k < a.top; ++k) {                       // (`need` slices have up to `top` keys that reach it, the others fewer than q)
             const skey key = keys[k];
             if (key < bound) break;
             list[atomicAdd(&count, 1)] = key;
@@ -354,9 +370,11 @@ constexpr int WHOLE = 32768;                    // scores that 16 waves hold
 constexpr int SLICE = 8192;                     // 4 waves
 
 // how a row is cut: few rows of up to 32768 scores stay whole, which saves the second launch (the 256 CUs hold two blocks of 16 waves each);
-// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 88 us, slices 71 + 7; 8192 x 131072: 557, 522 + 13)
+// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 88 us, slices 71 + 7; 8192 x 131072: 557, 522 + 13),
+// half as long where there would be fewer than half as many as CUs (1 x 131072 fp32: 7.0 -> 6.2 us)
 inline void cut(long long rows, int v, int &nsplit, int &slice) {
     nsplit = v <= WHOLE && rows <= 512 ? 1 : (v + SLICE - 1) / SLICE;
+    if (nsplit > 1 && nsplit <= 128 && rows * nsplit <= 128) nsplit = (v + SLICE / 2 - 1) / (SLICE / 2);
     slice = ((v + nsplit - 1) / nsplit + 7) & ~7;
     nsplit = (v + slice - 1) / slice;
 }
