@@ -393,7 +393,7 @@ template <bool Q8> int launch_fwd(int dtype, const FwdArgs &a, void *stream) {
 
 extern "C" int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr,
                                 const void *w, float eps, void *s, void *y, float *rstd, void *stream) {
-    if (rows < 0 || d <= 0 || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
+    if (rows < 0 || d <= 0 || d > I2P_MAX_ROW || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
     if (!x || !y) return I2P_ERR_BAD_ARG;
     return launch_fwd<false>(dtype, FwdArgs{rows, d, wdtype, (const char *)x, ldx, (const char *)res, ldr, w, eps, (char *)s, (char *)y, rstd, 0,
@@ -402,7 +402,7 @@ extern "C" int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, co
 
 extern "C" int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr,
                                const void *w, float eps, int group, void *s, unsigned char *q, float *scale, void *stream) {
-    if (rows < 0 || d <= 0 || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
+    if (rows < 0 || d <= 0 || d > I2P_MAX_ROW || !types_ok(dtype, wdtype) || ldx < d || (res && ldr < d) || (res != nullptr) != (s != nullptr)) return I2P_ERR_BAD_ARG;
     if (group != 0 && (group < 32 || group > 512 || (group & (group - 1)))) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
     if (!x || !q || !scale) return I2P_ERR_BAD_ARG;
@@ -414,7 +414,7 @@ extern "C" long long i2p_rms_norm_bwd_scratch(long long rows, int d) { return ro
 
 extern "C" int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, const void *s, long long lds, const void *gy, long long ldgy,
                                 const void *gs, long long ldgs, const void *w, const float *rstd, void *dx, void *dw, void *scratch, void *stream) {
-    if (rows <= 0 || d <= 0 || !types_ok(dtype, wdtype) || lds < d || ldgy < d || (gs && ldgs < d)) return I2P_ERR_BAD_ARG;
+    if (rows <= 0 || d <= 0 || d > I2P_MAX_ROW || !types_ok(dtype, wdtype) || lds < d || ldgy < d || (gs && ldgs < d)) return I2P_ERR_BAD_ARG;
     if (!s || !gy || !rstd || !dx || (dw && !scratch)) return I2P_ERR_BAD_ARG;
     const BwdArgs a{rows, d, wdtype, (const char *)s, lds, (const char *)gy, ldgy, (const char *)gs, ldgs, w, rstd, (char *)dx,
                     dw ? (float *)scratch : nullptr};

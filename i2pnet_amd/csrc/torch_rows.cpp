@@ -86,7 +86,7 @@ struct Rows {
                         x.device(), ")");
         TORCH_CHECK(x.dim() > 0 && x.size(-1) > 0, what, " must have rows of at least one element (got ", x.sizes(), ")");
         d = x.size(-1);
-        TORCH_CHECK(d <= INT_MAX, what, ": rows of ", d, " elements are too long");
+        TORCH_CHECK(d <= I2P_MAX_ROW, what, ": rows of ", d, " elements are too long");
         n = x.numel() / d;
         ld = d;
         t = x;
@@ -168,6 +168,7 @@ std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor &s, const OptTensor
     TORCH_CHECK(rstd.is_contiguous() && rstd.scalar_type() == at::kFloat && rstd.numel() == a.n && rstd.device() == s.device(), "rstd must be float32 [", a.n, "]");
     Tensor dx = at::empty(gy.sizes(), gy.options());
     OptTensor dw, scratch;
+    TORCH_CHECK(!need_dw || weight, "rms_norm_backward: the weight's gradient is wanted, but there is no weight");
     if (need_dw) dw = a.n ? at::empty_like(*weight) : at::zeros_like(*weight);
     if (a.n == 0) return {dx, dw};
     if (need_dw) scratch = at::empty({abi.rms_norm_bwd_scratch(a.n, (int)a.d)}, gy.options().dtype(at::kByte));
@@ -301,6 +302,8 @@ std::vector<Tensor> grad_list(const py::object &parameters) {
         TORCH_CHECK(THPVariable_Check(o), "parameters (leaves) or gradient tensors are wanted (got ", Py_TYPE(o)->tp_name, ")");
         const Tensor &t = THPVariable_Unpack(o);
         if (Py_TYPE(o) == (PyTypeObject *)THPVariableClass && !t.requires_grad()) { grads.push_back(t); return; }
+        TORCH_CHECK(t.requires_grad() || !ParameterClass || PyObject_IsInstance(o, ParameterClass) == 1,
+                    "parameters (leaves) or gradient tensors are wanted (got ", Py_TYPE(o)->tp_name, " without a gradient)");
         TORCH_CHECK(t.is_leaf(), "parameters (leaves) or gradient tensors are wanted (got a tensor that an operation made and that requires a gradient)");
         if (t.grad().defined()) grads.push_back(t.grad());
     };
@@ -312,6 +315,7 @@ std::vector<Tensor> grad_list(const py::object &parameters) {
 
 // total norm f32 0-d of a list that is not empty; no max_norm: nothing is clipped
 Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optional<double> max_norm, const OptTensor &out) {
+    TORCH_CHECK(!grads.empty(), "clip_grad_norm: no gradients");
     const auto device = grads[0].device();
     const int n = (int)grads.size();
     std::vector<const void *> ptrs(n);

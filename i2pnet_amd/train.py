@@ -173,11 +173,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative (got {max_norm})")
     if error_if_nonfinite:
-        parameters = _grad_list(parameters)
-        total = ops.rows().clip_parameters(parameters, kind, None, None)
-        if total is not None and not bool(torch.isfinite(total)):
+        grads = _grad_list(parameters)
+        if grads and not bool(torch.isfinite(ops.rows().clip_grad_norm(grads, kind, None, None))):
             raise RuntimeError("the global norm of the gradients is not finite: they were not clipped")
-    total = ops.rows().clip_parameters(parameters, kind, max_norm, out)
+        total = ops.rows().clip_grad_norm(grads, kind, max_norm, out) if grads else None
+    else:
+        total = ops.rows().clip_parameters(parameters, kind, max_norm, out)
     if total is None:
         if out is not None and out.numel():
             raise RuntimeError("out must be empty: there is no gradient")

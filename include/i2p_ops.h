@@ -705,16 +705,18 @@ int i2p_kitti_image_build(int B, int out_h, int out_w, const void *table, float 
 
 /* ---------------------------------------------------------------------------------------------
  * Row operators of a training or matching step (not in the reference): any width, rows of pitch ld >= width (elements), storage types
- * I2P_F32 / I2P_BF16 / I2P_F16, fp32 arithmetic, 1-byte alignment beyond the element's own not required.  Results are reproducible.
+ * I2P_F32 / I2P_BF16 / I2P_F16, fp32 arithmetic, no alignment beyond the element's own.  Results are reproducible.  Sizes outside what is said
+ * here, NULL pointers with work and pitches below the width are I2P_ERR_BAD_ARG; no rows is no work.
  *
  * Root-mean-square norm with the residual's addition: s [rows,d] = round(x + res) (res, s both NULL: the norm is of x itself),
- * rstd f32 [rows] = 1/sqrt(mean(s^2) + eps) (NULL: not wanted), y [rows,d] = round(s * rstd * w); w [d] of type wdtype (I2P_F32 or
+ * d <= I2P_MAX_ROW, rstd f32 [rows] = 1/sqrt(mean(s^2) + eps) (NULL: not wanted), y [rows,d] = round(s * rstd * w); w [d] of type wdtype (I2P_F32 or
  * dtype), NULL = ones.  s, y are dense.
  * _q8: q u8 [rows,d] = OCP e4m3 bits of s * rstd * w / scale, scale f32 [rows, ceil(d / group)] = max |s * rstd * w| / 448 over the group's
  * columns (1 where they are all zero); group a power of two, 32 .. 512, or 0 = the whole row.  A group with a NaN or inf has scale inf.
  * _bwd: gy [rows,d], gs (gradient of s, NULL = none) -> dx [rows,d] (dense; the gradient of x and of res), dw [d] of type wdtype (NULL: not
  * wanted); s, rstd as the forward left them; scratch: i2p_rms_norm_bwd_scratch(rows, d) bytes, needed with dw.
  * --------------------------------------------------------------------------------------------- */
+#define I2P_MAX_ROW (1 << 30)
 int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr, const void *w,
                      float eps, void *s, void *y, float *rstd, void *stream);
 int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr, const void *w,

@@ -90,6 +90,15 @@ def test_clip_grad_norm_output_must_not_overlap():
             clip([P, P + 1024], [4, 4], [0, 0], out=out)
 
 
+def test_rows_too_long():
+    d = (1 << 30) + 1
+    for name, args in (("i2p_rms_norm_fwd", (1, d, 1, 0, P, d, None, 0, None, 1e-6, None, P, None)),
+                       ("i2p_rms_norm_q8", (1, d, 1, 0, P, d, None, 0, None, 1e-6, 0, None, P, P)),
+                       ("i2p_rms_norm_bwd", (1, d, 1, 0, P, d, P, d, None, 0, None, P, P, None, None))):
+        with pytest.raises(_lib.I2POpsError, match=BAD):
+            call(name, *args)
+
+
 def test_scratch_sizes():
     n = (C.c_longlong * 3)(1, 0, (1 << 31) + 5)
     assert _lib.helper("i2p_grad_norm_scratch", 3, C.cast(n, C.c_void_p)) >= 8
@@ -116,6 +125,17 @@ def test_host_tensors_and_types_are_refused():
         train.clip_grad_norm_([(x.clone().requires_grad_(True) * 2)], 1.0)
     with pytest.raises(RuntimeError, match="leaves"):
         train.clip_grad_norm_([3.0], 1.0)
+
+
+def test_other_tensor_classes_are_refused_as_gradients():
+    class Other(torch.Tensor):
+        pass
+    with pytest.raises(RuntimeError, match="wanted"):
+        train._grad_list([torch.zeros(3).as_subclass(Other)])
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.rows().clip_grad_norm([], 0, 1.0, None)
+    with pytest.raises(RuntimeError, match="cuda"):
+        ops.rows().rms_norm_backward(torch.zeros(2, 3), None, torch.zeros(2), torch.zeros(2, 3), None, True)
 
 
 def test_lists_of_parameters():

@@ -691,3 +691,73 @@ def test_what_a_backward_pass_needs_may_not_be_changed():
     train.clip_grad_norm_([b.detach()], 1.0)                # clipping counts as a change too
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_a_captured_training_pass():
+    """forward and backward through autograd in a graph, replayed on new inputs with eager passes between"""
+    x, w = torch.zeros(64, 130, device=DEV, requires_grad=True), torch.ones(130, device=DEV, requires_grad=True)
+    ids = torch.zeros(64, dtype=torch.long, device=DEV)
+
+    def one():
+        y, s = modules.rms_norm(x, w, residual=x)
+        o = loss.token_logprobs(y, ids, top=2)
+        g = list(torch.autograd.grad(-o.logp.mean() + 0.1 * o.entropy.mean() + s.square().mean(), [x, w]))
+        return g + [train.clip_grad_norm_(g, 1e-3), o.logp.detach(), o.top_ids]
+
+    def fill(seed):
+        with torch.no_grad():
+            x.copy_(rnd(64, 130, seed=seed))
+        ids.copy_(torch.randint(0, 130, (64,), generator=torch.Generator().manual_seed(seed)))
+    fill(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = one()
+    for k in range(3):
+        fill(k + 1)
+        want = [t.clone() for t in one()]
+        graph.replay()
+        one()
+        torch.cuda.synchronize()
+        for p, q in zip(outs, want):
+            assert torch.equal(p, q)
+
+
+def test_gradients_that_carry_a_graph_can_be_clipped():
+    a = rnd(40, seed=1).to(DEV).requires_grad_(True)
+    (g,) = torch.autograd.grad((a ** 3).sum(), a, create_graph=True)
+    b = torch.nn.Parameter(torch.zeros(40, device=DEV))
+    b.grad = g
+    want = g.detach().clone()
+    n = train.clip_grad_norm_([b], 1.0, error_if_nonfinite=True)
+    assert abs(float(n) / float(want.double().norm()) - 1) < 2 * U
+    within(b.grad, want.double() / (want.double().norm() + 1e-6), 8 * U * want.abs(), "clipped")
+
+
+def test_reads_and_writes_between_guards():
+    """every operator on views in the middle of larger buffers: what lies around them keeps its bits, at each width's last vector"""
+    for dtype in TYPES:
+        for d in (1, 5, 8, 63, 65, 519, 2049, 4103):
+            pad = 24
+            buf = torch.full((3, d + 2 * pad), 1.0, dtype=dtype, device=DEV)
+            x = buf[:, pad:pad + d]
+            x.copy_(rnd(3, d, dtype=dtype, seed=d))
+            keep = buf.clone()
+            ids = torch.zeros(3, dtype=torch.long, device=DEV)
+            leaf = x.detach().requires_grad_(True)
+            y, s = modules.rms_norm(leaf, None, residual=leaf)
+            o = loss.token_logprobs(leaf, ids, top=min(d, 4))
+            torch.autograd.grad(y.float().sum() + s.float().sum() + o.logp.sum(), leaf)
+            modules.rms_norm_q8(x, None, group=32)
+            assert torch.equal(buf, keep)
+            flat = buf.view(-1)
+            views = [flat[k * (d + 2 * pad) + pad:k * (d + 2 * pad) + pad + d] for k in range(3)]
+            train.clip_grad_norm_(views, 1e-2)
+            mask = torch.ones_like(buf, dtype=torch.bool)
+            mask[:, pad:pad + d] = False
+            assert torch.equal(buf[mask], keep[mask])
