@@ -125,20 +125,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
             for (int e = 0; e < VE; ++e) { const unsigned b = __float_as_uint(f[e] * rstd * w[e]) & 0x7fffffffu; if (c.counts(e, d) && b > m[j]) m[j] = b; }
             all = m[j] > all ? m[j] : all;
         }
-        // a group of columns is a run of group / VE lanes of one vector number (all TPR of a short row)
-        const int lanes = a.group ? min(a.group / VE, TPR) : 0, ng = a.group ? (d + a.group - 1) / a.group : 1;
-        if (!a.group) all = row_reduce<TPR>(all, mred, Max{});
+        // a group of columns is a run of group / VE <= TPR lanes of one vector number, or the whole row
+        const bool whole = !a.group || a.group >= TPR * NV * VE;
+        const int lanes = whole ? 0 : a.group / VE, ng = whole ? 1 : (d + a.group - 1) / a.group;
+        if (whole) all = row_reduce<TPR>(all, mred, Max{});
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const Col<DT, TINY> c = col(j);
             unsigned b = all;
-            if (a.group) {
+            if (!whole) {
                 b = m[j];
                 for (int o = lanes >> 1; o > 0; o >>= 1) { const unsigned u = (unsigned)__shfl_xor((int)b, o, 64); b = u > b ? u : b; }
             }
             if (!c.in) continue;
             const float sc = scale_of(b), inv = 1.f / sc;
-            if (a.group ? (t & (lanes - 1)) == 0 : (t | j) == 0) a.scale[row * ng + (a.group ? (j * TPR + t) * VE / a.group : 0)] = sc;
+            if (whole ? (t | j) == 0 : (t & (lanes - 1)) == 0) a.scale[row * ng + (whole ? 0 : (j * TPR + t) * VE / a.group)] = sc;
             float f[VE], w[VE];
             unpack<DT>(v[j], f);
             ld_weight<DT>(a.w, a.wdtype, c, d, w);

@@ -185,6 +185,22 @@ def test_rms_norm_q8(dtype, rows, d, group, residual):
         assert torch.equal(out[2].cpu(), s)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("group", [32, 64, 128, 256, 512])
+@pytest.mark.parametrize("d", [33, 64, 96, 100, 129, 200, 256, 257, 300, 500, 511, 513, 1000, 1030, 2100])
+def test_rms_norm_q8_every_group_of_narrow_rows(dtype, group, d):
+    x, w = rnd(37, d, dtype=dtype, seed=d), 1 + rnd(d, seed=3) * 0.1
+    q, scale = modules.rms_norm_q8(x.to(DEV), w.to(DEV), eps=1e-5, group=group)
+    _, y = norm64(x, None, w, 1e-5)
+    ng = -(-d // group)
+    want = torch.nn.functional.pad(y.abs(), (0, ng * group - d)).view(37, ng, group).amax(-1) / 448
+    rel = (chain(d) + 12) * U
+    within(scale, want, rel * want, "scale")
+    cols = scale.cpu().double().repeat_interleave(group, 1)[:, :d]
+    err = (q.cpu().double() * cols - y).abs()
+    assert float((err - (2.0 ** -4 * (1 + rel) * y.abs()).clamp_min(2.0 ** -10 * 1.01 * cols) - 2 * rel * y.abs()).max()) <= 0
+
+
 def test_rms_norm_q8_special_rows():
     x = rnd(6, 64, seed=1)
     x[1] = 0
