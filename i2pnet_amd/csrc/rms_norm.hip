@@ -18,9 +18,8 @@ constexpr int DW_COLS = 32, DW_LANES = 32;      // dw reduction: columns and row
 
 // sum (or maximum of non-negative values' bits) over the TPR threads of a row; every one gets it.  A block-wide row uses red[waves]; calls
 // alternate between two such arrays, so that one barrier each is enough
-template <int TPR, class V, class Op> __device__ __forceinline__ V row_reduce(V v, V *red, Op op) {
-#pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v = op(v, (V)__shfl_xor(v, o, 64));
+template <int TPR, class Op> __device__ __forceinline__ unsigned row_reduce(unsigned v, unsigned *red, Op op) {
+    v = lanes_reduce<(TPR < 64 ? TPR : 64)>(v, op);
     if constexpr (TPR > 64) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
@@ -30,8 +29,7 @@ template <int TPR, class V, class Op> __device__ __forceinline__ V row_reduce(V 
     }
     return v;
 }
-struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
-struct Max { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; } };
+template <int TPR> __device__ __forceinline__ float row_sum(float v, unsigned *red) { return __uint_as_float(row_reduce<TPR>(__float_as_uint(v), red, AddF{})); }
 
 // the weights of a vector of columns (ones where there is no weight)
 template <int DT, bool TINY> __device__ __forceinline__ void ld_weight(const void *w, int wdtype, const Col<DT, TINY> &c, int d, float (&f)[i2p_vec(DT)]) {
@@ -65,7 +63,7 @@ __device__ __forceinline__ float scale_of(unsigned bits) {
 template <int DT, int TPR, int NV, bool TINY, bool Q8>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4) void rms_fwd_kernel(FwdArgs a) {
     constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT), BLOCK = TPR < 256 ? 256 : TPR;
-    __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+    __shared__ unsigned red[TPR > 64 ? TPR / 64 : 1];
     __shared__ unsigned mred[TPR > 64 ? TPR / 64 : 1];
     const long long row = (long long)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
     if (TPR < BLOCK && row >= a.rows) return;                   // (a block-wide row always exists)
@@ -99,7 +97,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc += e >= c.skip ? f[e] * f[e] : 0.f;        // (what is past the row was read as 0)
     }
-    const float rstd = 1.f / sqrtf(row_reduce<TPR>(acc, red, Add{}) / (float)d + a.eps);
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(acc, red) / (float)d + a.eps);
     if constexpr (!Q8) {
         if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
@@ -128,14 +126,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
         // a group of columns is a run of group / VE <= TPR lanes of one vector number, or the whole row
         const bool whole = !a.group || a.group >= TPR * NV * VE;
         const int lanes = whole ? 0 : a.group / VE, ng = whole ? 1 : (d + a.group - 1) / a.group;
-        if (whole) all = row_reduce<TPR>(all, mred, Max{});
+        if (whole) all = row_reduce<TPR>(all, mred, MaxU{});
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const Col<DT, TINY> c = col(j);
             unsigned b = all;
             if (!whole) {
                 b = m[j];
-                for (int o = lanes >> 1; o > 0; o >>= 1) { const unsigned u = (unsigned)__shfl_xor((int)b, o, 64); b = u > b ? u : b; }
+                b = lanes == 64 ? lanes_reduce<64>(b, MaxU{}) : lanes == 32 ? lanes_reduce<32>(b, MaxU{}) : lanes == 16 ? lanes_reduce<16>(b, MaxU{})
+                    : lanes == 8 ? lanes_reduce<8>(b, MaxU{}) : lanes_reduce<4>(b, MaxU{});
             }
             if (!c.in) continue;
             const float sc = scale_of(b), inv = 1.f / sc;
@@ -167,7 +166,7 @@ struct BwdArgs {
 template <int DT, int TPR, int NV, bool TINY>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(BwdArgs a) {
     constexpr int VE = i2p_vec(DT), ES = i2p_esize(DT), BLOCK = TPR < 256 ? 256 : TPR, RPB = BLOCK / TPR;
-    __shared__ float red[2][TPR > 64 ? TPR / 64 : 1];
+    __shared__ unsigned red[2][TPR > 64 ? TPR / 64 : 1];
     __shared__ float cols[RPB > 1 ? BLOCK * VE : 1];
     const int t = threadIdx.x % TPR, d = a.d;
     auto col = [&](int j) { return Col<DT, TINY>(j * TPR + t, d); };
@@ -193,7 +192,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(BwdArgs 
 #pragma unroll
             for (int e = 0; e < VE; ++e) { const float p = g[e] * (f[e] * rstd); dw[j][e] += p; acc += e >= c.skip ? p * w[e] : 0.f; }
         }
-        const float mean = row_reduce<TPR>(acc, red[flip], Add{}) / (float)d;
+        const float mean = row_sum<TPR>(acc, red[flip]) / (float)d;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float f[VE], g[VE], w[VE], h[VE] = {};
@@ -285,7 +284,7 @@ template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_ke
                 const int hi = min(d, (g + 1) * a.group);
                 unsigned m = 0u;
                 for (int i = g * a.group + lane; i < hi; i += 64) { const unsigned b = __float_as_uint(val(i)) & 0x7fffffffu; m = b > m ? b : m; }
-                m = row_reduce<64>(m, (unsigned *)nullptr, Max{});
+                m = row_reduce<64>(m, (unsigned *)nullptr, MaxU{});
                 const float sc = scale_of(m), inv = 1.f / sc;
                 if (lane == 0) a.scale[row * ng + g] = sc;
                 for (int i = g * a.group + lane; i < hi; i += 64) a.q[row * d + i] = (unsigned char)e4m3_pack4(val(i) * inv, 0.f, 0.f, 0.f);
@@ -294,7 +293,7 @@ template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_ke
             unsigned m = 0u;
             for (int i = threadIdx.x; i < d; i += LT) { const unsigned b = __float_as_uint(val(i)) & 0x7fffffffu; m = b > m ? b : m; }
             __syncthreads();
-            m = row_reduce<LT>(m, (unsigned *)red, Max{});
+            m = row_reduce<LT>(m, (unsigned *)red, MaxU{});
             const float sc = scale_of(m), inv = 1.f / sc;
             if (threadIdx.x == 0) a.scale[row] = sc;
             for (int i = threadIdx.x; i < d; i += LT) a.q[row * d + i] = (unsigned char)e4m3_pack4(val(i) * inv, 0.f, 0.f, 0.f);

@@ -61,8 +61,8 @@ template <int DT, bool TINY = false> struct Col {
         at = TINY ? i : min(i, d - VE);
         skip = TINY ? 0 : i - at;
     }
-    __device__ __forceinline__ uint4 load(const char *row, int d) const {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    __device__ __forceinline__ uint4 load(const char *row, int d, unsigned fill = 0u) const {
+        uint4 v = make_uint4(fill, fill, fill, fill);
         if (!in) return v;
         if (!TINY || at + VE <= d) __builtin_memcpy(&v, row + (long long)at * ES, 16);
         else {
@@ -94,11 +94,27 @@ template <int DT, bool TINY = false> struct Col {
     __device__ __forceinline__ bool counts(int e, int d) const { return in && e >= skip && (!TINY || at + e < d); }
 };
 
+// Butterfly reduction over groups of N = 2 .. 64 lanes; every lane gets the same bits.  Register moves only (DPP inside a row of 16 lanes, the
+// lane swaps of gfx950 above): a reduction through ds_bpermute is some thirty instructions and six LDS round trips
+template <int N, class Op> __device__ __forceinline__ unsigned lanes_reduce(unsigned v, Op op) {
+    if constexpr (N >= 2) v = op(v, i2p_dpp_u32<0xB1>(v));
+    if constexpr (N >= 4) v = op(v, i2p_dpp_u32<0x4E>(v));
+    if constexpr (N >= 8) v = op(v, i2p_dpp_u32<0x141>(v));
+    if constexpr (N >= 16) v = op(v, i2p_dpp_u32<0x140>(v));
+    if constexpr (N >= 32) { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); v = op(r[0], r[1]); }
+    if constexpr (N >= 64) { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); v = op(r[0], r[1]); }
+    return v;
+}
+struct AddF { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); } };
+struct MaxF { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); } };
+struct MaxU { __device__ __forceinline__ unsigned operator()(unsigned a, unsigned b) const { return a > b ? a : b; } };
+template <int N> __device__ __forceinline__ float lanes_sum(float v) { return __uint_as_float(lanes_reduce<N>(__float_as_uint(v), AddF{})); }
+template <int N> __device__ __forceinline__ float lanes_max(float v) { return __uint_as_float(lanes_reduce<N>(__float_as_uint(v), MaxF{})); }
+
 // sum / maximum over the block's waves; every thread gets the result.  red: one float per wave.  (All threads of the block call it; the
 // trailing barrier lets the caller use `red` again.)
 template <bool MAX> __device__ __forceinline__ float block_reduce(float v, float *red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const float u = __shfl_xor(v, o, 64); v = MAX ? fmaxf(v, u) : v + u; }
+    v = MAX ? lanes_max<64>(v) : lanes_sum<64>(v);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float t = red[0];

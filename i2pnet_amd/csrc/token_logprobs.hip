@@ -65,17 +65,6 @@ struct FwdArgs {
     skey *keys;                                // [rows][nsplit][top], best first
 };
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-
 // what a row's results are, from its maximum and sums; one thread
 __device__ __forceinline__ void finish_row(const FwdArgs &a, long long row, long long id, float xid, float c, float S, float U) {
     const bool empty = S == 0.f;
@@ -119,8 +108,8 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const Col<DT, TINY> c(j * T + t, n);
-        v[j] = c.load(x, n);
-        if (!c.in || c.skip || c.at + VE > n) {                 // what is not this vector's reads as -inf
+        v[j] = c.load(x, n, minus_inf<DT>());
+        if (c.skip || (TINY && c.in && c.at + VE > n)) {        // what is not this vector's reads as -inf
             float f[VE];
             unpack<DT>(v[j], f);
 #pragma unroll
@@ -141,16 +130,14 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     }
     hold(v);
     // 64 groups of W lanes
-    float g = most;
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor(g, o, 64));
+    float g = lanes_max<W>(most);
     if constexpr (W > 1) {
         if ((t & (W - 1)) == 0) gmax[t / W] = g;
         if (t == 0) count = 0;
         __syncthreads();
         g = gmax[lane];
     } else if (t == 0) count = 0;
-    const float m = wave_max(g), c = shift_of(m);
+    const float m = lanes_max<64>(g), c = shift_of(m);
     // the largest value, to 16 bits of its order, that at least `top` groups reach
     float least = -__builtin_inff();
     if (a.top) {
@@ -183,7 +170,7 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
         }
     }
     hold(v);
-    S = wave_sum(S); U = wave_sum(U);
+    S = lanes_sum<64>(S); U = lanes_sum<64>(U);
     if constexpr (W > 1) {
         if (lane == 0) { sums[0][wave] = S; sums[1][wave] = U; }
         __syncthreads();
@@ -280,7 +267,7 @@ __global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype)
         const long long i = row * a.ldx + id;
         xid = dtype == I2P_F32 ? ld1<I2P_F32>(a.x, i) : dtype == I2P_BF16 ? ld1<I2P_BF16>(a.x, i) : ld1<I2P_F16>(a.x, i);
     }
-    float m = wave_max(p.x);
+    float m = lanes_max<64>(p.x);
     if (lane == 0) sums[0][wave] = m;
     head[t] = mine;
     if (t == 0) { count = 0; bound = 0ull; }
@@ -288,7 +275,7 @@ __global__ __launch_bounds__(JT) void logprobs_join_kernel(FwdArgs a, int dtype)
 #pragma unroll
     for (int w = 0; w < JT / 64; ++w) m = fmaxf(m, sums[0][w]);
     const float c = shift_of(m), shift = p.x - c, f = __expf(shift);
-    float S = wave_sum(f * p.y), U = wave_sum(f * __builtin_fmaf(fmaxf(shift, -200.f), p.y, p.z));
+    float S = lanes_sum<64>(f * p.y), U = lanes_sum<64>(f * __builtin_fmaf(fmaxf(shift, -200.f), p.y, p.z));
     if (lane == 0) { sums[1][wave] = S; sums[2][wave] = U; }
     if (a.top && t < a.nsplit) {
         int rank = 0;
