@@ -7,7 +7,7 @@
 // A row without candidates (all -inf): logp -inf, H 0, gradient 0.  +inf or NaN in a row: logp, H, top_logp and the gradient are NaN.
 //
 // Forward: bound by the one read of the scores.  A row, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at
-// most 32 scores a thread), so that the true maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k best
+// most 32 scores a thread, 64 of the 16-bit types), so that the true maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k best
 // in the workspace and a second launch joins them.
 // Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those (to 16 bits) is a value that at least k scores reach
 // and that few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow that list
@@ -91,7 +91,7 @@ template <int N> __device__ __forceinline__ void hold(uint4 (&v)[N]) {
 }
 
 template <int DT, int W, int E>
-__global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8) void logprobs_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W < 16) ? 6 : 8) void logprobs_fwd_kernel(FwdArgs a) {
     constexpr int T = 64 * W, VE = i2p_vec(DT), NV = E / VE;
     constexpr bool TINY = T * E == 512;
     __shared__ float gmax[64], sums[2][W];
@@ -104,7 +104,6 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     const char *x = a.x + (row * a.ldx + lo) * i2p_esize(DT);
     if (id == a.ignore) { if (a.nsplit == 1) skip_row(a, row); return; }
     uint4 v[NV];
-    float vmax[NV], most = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const Col<DT, TINY> c(j * T + t, n);
@@ -119,6 +118,7 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     }
     float xid = 0.f;
     if (a.nsplit == 1 && t == 0 && id >= 0 && id < a.v) xid = ld1<DT>(x, id);
+    float vmax[NV], most = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         float f[VE];
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
     };
     if constexpr (W == 1) __syncthreads();                      // (`count`)
     const bool plain = S == S;                                  // no NaN, no +inf
-    unsigned bits = 0u;                                         // which of the thread's scores reach the bound
+    unsigned long long bits = 0ull;                             // which of the thread's scores reach the bound
     if (plain && most >= least) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -200,19 +200,19 @@ __global__ __launch_bounds__(64 * W, DT == I2P_F32 && E == 32 && W < 16 ? 6 : 8)
             unpack<DT>(v[j], f);
 #pragma unroll
             for (int e = 0; e < VE; ++e)
-                if (f[e] >= least && (least > -__builtin_inff() || col.counts(e, n))) bits |= 1u << (j * VE + e);
+                if (f[e] >= least && (least > -__builtin_inff() || col.counts(e, n))) bits |= 1ull << (j * VE + e);
         }
     }
     for (;;) {                                                  // one of each lane a turn; its value is read again, from the caches
-        const skey has = __ballot(bits != 0u);
+        const skey has = __ballot(bits != 0ull);
         if (!has) break;
         int base = 0;
         if (lane == 0) base = atomicAdd(&count, __popcll(has));
         base = __builtin_amdgcn_readfirstlane(base);
         if (base >= LIST) break;
         if (bits) {
-            const int i = __ffs(bits) - 1, at = base + __popcll(has & ((1ull << lane) - 1ull));
-            bits &= bits - 1u;
+            const int i = __ffsll(bits) - 1, at = base + __popcll(has & ((1ull << lane) - 1ull));
+            bits &= bits - 1ull;
             const int col = Col<DT, TINY>(i / VE * T + t, n).at + i % VE;
             if (at < LIST) list[at] = key_of(ld1<DT>(x, col), (unsigned)(lo + col));
         }
@@ -354,14 +354,17 @@ template <class F> void by_type(int dtype, F f) {
 }
 
 constexpr int WHOLE = 32768;                    // scores that 16 waves hold
+constexpr int FEW = 4096;                       // a slice where blocks are few
 constexpr int SLICE = 8192;                     // 4 waves
 
 // how a row is cut: few rows of up to 32768 scores stay whole, which saves the second launch (the 256 CUs hold two blocks of 16 waves each);
-// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 88 us, slices 71 + 7; 8192 x 131072: 557, 522 + 13),
-// half as long where there would be fewer than half as many as CUs (1 x 131072 fp32: 7.0 -> 6.2 us)
-inline void cut(long long rows, int v, int &nsplit, int &slice) {
+// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 88 us, slices of 8192 71 + 7; 8192 x 131072: 557,
+// 522 + 13), shorter ones where there would be fewer than half as many as CUs (1 x 131072 fp32: 7.0 -> 6.2 us) and, of the 16-bit types, longer
+// ones where they still fill the chip ten times (8192 x 131072: 492 -> 455 us; 4096 x 32000, which is five times: 72 -> 80)
+inline void cut(long long rows, int v, int dtype, int &nsplit, int &slice) {
     nsplit = v <= WHOLE && rows <= 512 ? 1 : (v + SLICE - 1) / SLICE;
-    if (nsplit > 1 && nsplit <= 128 && rows * nsplit <= 128) nsplit = (v + SLICE / 2 - 1) / (SLICE / 2);
+    if (dtype != I2P_F32 && nsplit > 1 && rows * ((nsplit + 1) / 2) >= 16384) nsplit = (v + 2 * SLICE - 1) / (2 * SLICE);
+    if (nsplit > 1 && rows * nsplit <= 128 && v <= FEW * JT) nsplit = (v + FEW - 1) / FEW;
     slice = ((v + nsplit - 1) / nsplit + 7) & ~7;
     nsplit = (v + slice - 1) / slice;
 }
@@ -372,10 +375,10 @@ inline bool sizes_ok(long long rows, int v, int dtype, long long ldx) {
 
 }  // namespace
 
-extern "C" long long i2p_token_logprobs_scratch(long long rows, int v, int, int top) {
+extern "C" long long i2p_token_logprobs_scratch(long long rows, int v, int dtype, int top) {
     if (rows <= 0 || v <= 0 || v > I2P_MAX_CANDIDATES || top < 0 || top > I2P_MAX_TOP) return 0;
     int nsplit, slice;
-    cut(rows, v, nsplit, slice);
+    cut(rows, v, dtype, nsplit, slice);
     return nsplit == 1 ? 0 : rows * nsplit * (16 + 8ll * top);
 }
 
@@ -385,7 +388,7 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
     if (rows == 0) return 0;
     if (!x || !ids || !logp || !entropy || !stat || (top && (!top_logp || !top_ids))) return I2P_ERR_BAD_ARG;
     int nsplit, slice;
-    cut(rows, v, nsplit, slice);
+    cut(rows, v, dtype, nsplit, slice);
     if (nsplit > 1 && !scratch) return I2P_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
     const long long most = (1 << 21) / nsplit;                  // rows of a launch: a grid has fewer than 2^32 threads
@@ -400,6 +403,7 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
         else if (slice <= 2048) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 32>), grid, dim3(64), 0, st, a);
         else if (slice <= 4096) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 16>), grid, dim3(256), 0, st, a);
         else if (slice <= SLICE) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 32>), grid, dim3(256), 0, st, a);
+        else if (DT != I2P_F32 && slice <= 2 * SLICE && (nsplit > 1 || rows > 512)) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, (DT == I2P_F32 ? 32 : 64)>), grid, dim3(256), 0, st, a);
         else if (slice <= 16384) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 16, 16>), grid, dim3(1024), 0, st, a);
         else hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 16, 32>), grid, dim3(1024), 0, st, a);
         if (nsplit > 1) hipLaunchKernelGGL(logprobs_join_kernel, dim3((unsigned)k), dim3(JT), 0, st, a, dtype);
