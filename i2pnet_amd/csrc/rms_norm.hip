@@ -224,9 +224,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(BwdArgs 
         }
         if (RPB == 1 || threadIdx.x < TPR) {
             const Col<DT, TINY> c = col(j);
+            if (c.in && !c.skip && c.at + VE <= d) __builtin_memcpy(out + c.at, dw[j], 4 * VE);
+            else
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-                if (c.counts(e, d)) out[c.at + e] = dw[j][e];
+                for (int e = 0; e < VE; ++e)
+                    if (c.counts(e, d)) out[c.at + e] = dw[j][e];
         }
     }
 }
@@ -340,7 +342,7 @@ inline long long bwd_blocks(long long rows, int d, int threads) {
 }
 
 // f(DT, TPR, NV) for rows of d elements; false: the row does not fit the registers of a block
-template <int DT, class F> bool by_width(int d, F f) {
+template <int DT, bool BWD, class F> bool by_width(int d, F f) {
     using std::integral_constant;
     const long long n = ((long long)d + i2p_vec(DT) - 1) / i2p_vec(DT);
 #define I2P_ROW(TPR, NV, TINY) { f(integral_constant<int, DT>{}, integral_constant<int, TPR>{}, integral_constant<int, NV>{}, std::bool_constant<TINY>{}); return true; }
@@ -351,6 +353,13 @@ template <int DT, class F> bool by_width(int d, F f) {
     if (n <= 64) I2P_ROW(64, 1, false)
     if (n <= 128) I2P_ROW(64, 2, false)
     if (n <= 256) I2P_ROW(256, 1, false)
+    if constexpr (BWD) {
+        // the weight gradients double the registers of a vector: more threads with one vector each (8192 x 4096 bf16 as 256 x 2: 55.9 us,
+        // 512 x 1: 52.6; 4000 x 8000 as 512 x 2: 76.6, 1024 x 1: 50.6), unless many of them would have none (15000 x 2100: 55.6, 62.1)
+        if (n <= 384) I2P_ROW(256, 2, false)
+        if (n <= 512) I2P_ROW(512, 1, false)
+        if (n <= 1024) I2P_ROW(1024, 1, false)
+    }
     if (n <= 512) I2P_ROW(256, 2, false)
     if (n <= 768) I2P_ROW(256, 3, false)
     if (n <= 1024) I2P_ROW(512, 2, false)
@@ -359,15 +368,15 @@ template <int DT, class F> bool by_width(int d, F f) {
 #undef I2P_ROW
     return false;
 }
-template <class F, class G> void by_row(int dtype, int d, F f, G longer, int group = 0) {
+template <bool BWD, class F, class G> void by_row(int dtype, int d, F f, G longer, int group = 0) {
     // (512 columns of fp32 are two waves' vectors: such groups take the long-row kernel unless they cover the row)
-    if (dtype == I2P_F32) { if ((group > 256 && d > 256) || !by_width<I2P_F32>(d, f)) longer(std::integral_constant<int, I2P_F32>{}); }
-    else if (dtype == I2P_BF16) { if (!by_width<I2P_BF16>(d, f)) longer(std::integral_constant<int, I2P_BF16>{}); }
-    else if (!by_width<I2P_F16>(d, f)) longer(std::integral_constant<int, I2P_F16>{});
+    if (dtype == I2P_F32) { if ((group > 256 && d > 256) || !by_width<I2P_F32, BWD>(d, f)) longer(std::integral_constant<int, I2P_F32>{}); }
+    else if (dtype == I2P_BF16) { if (!by_width<I2P_BF16, BWD>(d, f)) longer(std::integral_constant<int, I2P_BF16>{}); }
+    else if (!by_width<I2P_F16, BWD>(d, f)) longer(std::integral_constant<int, I2P_F16>{});
 }
 
 template <bool Q8> int launch_fwd(int dtype, const FwdArgs &a, void *stream) {
-    by_row(dtype, a.d, [&](auto dt, auto tpr, auto nv, auto tiny) {
+    by_row<false>(dtype, a.d, [&](auto dt, auto tpr, auto nv, auto tiny) {
         constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
         constexpr long long MOST = 1ll << 21;                   // blocks of a launch: a grid has fewer than 2^32 threads
         const long long es = i2p_esize(dt.value), ng = a.group ? (a.d + a.group - 1) / a.group : 1;
@@ -419,7 +428,7 @@ extern "C" int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, co
     const BwdArgs a{rows, d, wdtype, (const char *)s, lds, (const char *)gy, ldgy, (const char *)gs, ldgs, w, rstd, (char *)dx,
                     dw ? (float *)scratch : nullptr};
     long long nblk = 0;
-    by_row(dtype, d, [&](auto dt, auto tpr, auto nv, auto tiny) {
+    by_row<true>(dtype, d, [&](auto dt, auto tpr, auto nv, auto tiny) {
         constexpr int BLOCK = tpr.value < 256 ? 256 : tpr.value, RPB = BLOCK / tpr.value;
         nblk = bwd_blocks((rows + RPB - 1) / RPB, d, BLOCK);
         hipLaunchKernelGGL((rms_bwd_kernel<dt.value, tpr.value, nv.value, tiny.value>), dim3((unsigned)nblk), dim3(BLOCK), 0, (hipStream_t)stream, a);
