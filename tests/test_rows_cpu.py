@@ -78,7 +78,7 @@ def test_clip_grad_norm_refusals(args, what):
         clip(*args)
 
 
-@pytest.mark.parametrize("change", [dict(kind=2), dict(kind=-1), dict(limit=-1.0), dict(limit=math.nan), dict(scratch=None), dict(total=None), dict(n=-1)])
+@pytest.mark.parametrize("change", [dict(kind=2), dict(kind=-1), dict(limit=-1.0), dict(limit=math.nan), dict(scratch=None), dict(scratch=P + 8), dict(total=None), dict(n=-1)])
 def test_clip_grad_norm_argument_refusals(change):
     with pytest.raises(_lib.I2POpsError, match=BAD):
         clip([P], [4], [0], **change)

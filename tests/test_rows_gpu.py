@@ -512,6 +512,7 @@ def test_clip_grad_norm_large_values_and_parameters():
         if k in want:
             within(p.grad, want[k].double() * (0.25 / (n64 + 1e-6)), 8 * U * want[k].abs(), k)
     assert torch.equal(net[1].bias, kept)
+    assert float(train.clip_grad_norm_([torch.zeros(0, device=DEV)], 1.0)) == 0.0
     assert float(train.clip_grad_norm_([net[1].bias], 1.0)) == 0.0 and float(train.grad_norm([])) == 0.0
     single = torch.full((4,), 3.0, device=DEV)
     assert float(train.clip_grad_norm_(single, 7.0)) == 6.0 and single.eq(3).all()
