@@ -90,6 +90,8 @@ template <int DT, bool TINY = false> struct Col {
                 }
         }
     }
+    // the same past the caches (a whole vector of a row that is aligned)
+    __device__ __forceinline__ void store_stream(char *row, const uint4 &v) const { if (in) st_u4_stream(row + (long long)at * ES, v); }
     // does element `e` of the vector count (is it the row's, and not the previous vector's)?
     __device__ __forceinline__ bool counts(int e, int d) const { return in && e >= skip && (!TINY || at + e < d); }
 };

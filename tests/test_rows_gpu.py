@@ -778,3 +778,25 @@ def test_reads_and_writes_between_guards():
             mask = torch.ones_like(buf, dtype=torch.bool)
             mask[:, pad:pad + d] = False
             assert torch.equal(buf[mask], keep[mask])
+
+
+@pytest.mark.parametrize("rows,v,dtype", [(2100, 16384, torch.bfloat16), (1100, 16388, torch.float32), (1100, 16389, torch.float32)])
+def test_token_logprobs_gradient_past_the_caches(rows, v, dtype):
+    """gradients of 64 MB and more, which are written past the caches where rows start on 16 bytes: the same bits as row by row"""
+    x = torch.randn(rows, v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
+    ids = torch.randint(0, v, (rows,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    ids[5] = -100
+    ids[rows - 1] = v
+    leaf = x.clone().requires_grad_(True)
+    o = loss.token_logprobs(leaf, ids)
+    (d,) = torch.autograd.grad(o.logp.sum() + o.entropy.sum(), leaf)
+    assert not d[5].any() and torch.isnan(d[rows - 1]).all()
+    for lo in range(0, rows - 1, 100):
+        part = x[lo:lo + 100].clone().requires_grad_(True)
+        q = loss.token_logprobs(part, ids[lo:lo + 100])
+        hi = min(lo + 100, rows - 1)
+        (e,) = torch.autograd.grad(q.logp.sum() + q.entropy.sum(), part)
+        # (another number of rows may cut them otherwise, and sum in another order)
+        n = hi - lo
+        diff = (d[lo:hi].float() - e[:n].float()).abs()
+        assert float((diff - (2 * half_step(dtype) + 1000 * U) * e[:n].float().abs()).max()) <= 1e-6
