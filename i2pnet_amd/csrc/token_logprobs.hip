@@ -74,14 +74,14 @@ __device__ __forceinline__ void finish_row(const FwdArgs &a, long long row, long
     const float L = empty ? __builtin_inff() : logf(S);
     a.logp[row] = id < 0 || id >= a.v ? __builtin_nanf("") : (xid - c) - L;
     a.entropy[row] = empty ? 0.f : L - U / S;
-    a.stat[2 * row] = c; a.stat[2 * row + 1] = L;
+    if (a.stat) { a.stat[2 * row] = c; a.stat[2 * row + 1] = L; }
 }
 __device__ __forceinline__ void put_top(const FwdArgs &a, long long row, int rank, skey key, float c, float S) {
     a.top_logp[row * a.top + rank] = S == 0.f ? -__builtin_inff() : (score_of(key) - c) - logf(S);
     a.top_ids[row * a.top + rank] = col_of(key);
 }
 __device__ __forceinline__ void skip_row(const FwdArgs &a, long long row) {
-    if (threadIdx.x == 0) { a.logp[row] = 0.f; a.entropy[row] = 0.f; a.stat[2 * row] = 0.f; a.stat[2 * row + 1] = 0.f; }
+    if (threadIdx.x == 0) { a.logp[row] = 0.f; a.entropy[row] = 0.f; if (a.stat) a.stat[2 * row] = a.stat[2 * row + 1] = 0.f; }
     for (int k = threadIdx.x; k < a.top; k += blockDim.x) { a.top_logp[row * a.top + k] = -__builtin_inff(); a.top_ids[row * a.top + k] = -1; }
 }
 
@@ -391,7 +391,7 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
                                       float *logp, float *entropy, float *stat, float *top_logp, int64_t *top_ids, void *scratch, void *stream) {
     if (!sizes_ok(rows, v, dtype, ldx) || top < 0 || top > v || top > I2P_MAX_TOP) return I2P_ERR_BAD_ARG;
     if (rows == 0) return 0;
-    if (!x || !ids || !logp || !entropy || !stat || (top && (!top_logp || !top_ids))) return I2P_ERR_BAD_ARG;
+    if (!x || !ids || !logp || !entropy || (top && (!top_logp || !top_ids))) return I2P_ERR_BAD_ARG;
     int nsplit, slice;
     cut(rows, v, dtype, nsplit, slice);
     if (nsplit > 1 && (!scratch || ((uintptr_t)scratch & 15))) return I2P_ERR_BAD_ARG;
@@ -399,7 +399,7 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
     const long long most = (1 << 21) / nsplit;                  // rows of a launch: a grid has fewer than 2^32 threads
     for (long long r = 0; r < rows; r += most) by_type(dtype, [&](auto dt) {
         const long long k = rows - r < most ? rows - r : most;
-        const FwdArgs a{k, v, (const char *)x + r * ldx * i2p_esize(dtype), ldx, ids + r, ignore, top, logp + r, entropy + r, stat + 2 * r,
+        const FwdArgs a{k, v, (const char *)x + r * ldx * i2p_esize(dtype), ldx, ids + r, ignore, top, logp + r, entropy + r, stat ? stat + 2 * r : nullptr,
                         top_logp + r * top, top_ids + r * top, nsplit, slice, (float4 *)scratch + r * nsplit,
                         (skey *)((char *)scratch + rows * nsplit * 16) + r * nsplit * top};
         const dim3 grid((unsigned)(k * nsplit));

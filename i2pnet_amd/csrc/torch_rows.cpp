@@ -222,7 +222,7 @@ std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor &x, const OptTensor &w
 // ---- log probabilities -----------------------------------------------------------------------------------------------------------
 // -> logp, entropy, top_logp, top_ids, the scores as rows, ids (contiguous), stat
 using Logprobs = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
-Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t top, int64_t ignore_index) {
+Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t top, int64_t ignore_index, bool want_stat) {
     const Rows a(logits, "logits");
     TORCH_CHECK(ids.scalar_type() == at::kLong && ids.device() == logits.device() && ids.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                 "ids must be int64 ", logits.sizes().slice(0, logits.dim() - 1), " on ", logits.device(), " (got ", ids.scalar_type(), " ", ids.sizes(),
@@ -234,13 +234,14 @@ Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t
     const auto f32 = logits.options().dtype(at::kFloat);
     std::vector<int64_t> list = ids.sizes().vec();
     list.push_back(top);
-    Tensor logp = at::empty(ids.sizes(), f32), entropy = at::empty(ids.sizes(), f32), stat = at::empty({a.n, 2}, f32), top_logp = at::empty(list, f32),
+    Tensor logp = at::empty(ids.sizes(), f32), entropy = at::empty(ids.sizes(), f32), stat, top_logp = at::empty(list, f32),
            top_ids = at::empty(list, id.options());
+    if (want_stat) stat = at::empty({a.n, 2}, f32);
     OptTensor scratch;
     if (const int64_t bytes = abi.token_logprobs_scratch(a.n, (int)a.d, a.type, (int)top)) scratch = at::empty({bytes}, f32.dtype(at::kByte));
     const On on(logits.device());
     check(abi.token_logprobs_fwd(a.n, (int)a.d, a.type, a.t.data_ptr(), a.ld, id.data_ptr<int64_t>(), ignore_index, (int)top, logp.data_ptr<float>(),
-                                 entropy.data_ptr<float>(), stat.data_ptr<float>(), top_logp.data_ptr<float>(), top_ids.data_ptr<int64_t>(), ptr(scratch),
+                                 entropy.data_ptr<float>(), want_stat ? stat.data_ptr<float>() : nullptr, top_logp.data_ptr<float>(), top_ids.data_ptr<int64_t>(), ptr(scratch),
                                  on.stream()),
           "i2p_token_logprobs_fwd");
     return {logp, entropy, top_logp, top_ids, a.t, id, stat};
@@ -268,7 +269,7 @@ Tensor token_logprobs_backward(const Tensor &x2, const Tensor &ids, int64_t igno
 
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &ids, int64_t top, int64_t ignore_index) {
-        auto [logp, entropy, top_logp, top_ids, x2, id, stat] = token_logprobs_forward(logits, ids, top, ignore_index);
+        auto [logp, entropy, top_logp, top_ids, x2, id, stat] = token_logprobs_forward(logits, ids, top, ignore_index, true);
         ctx->set_materialize_grads(false);
         ctx->mark_non_differentiable({top_logp, top_ids});
         ctx->save_for_backward({x2, id, stat, entropy});
@@ -287,7 +288,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, const Tensor &ids, int64_t top, int64_t ignore_index) {
     if (!wants_grad(logits, std::nullopt, std::nullopt)) {
-        auto [logp, entropy, top_logp, top_ids, x2, id, stat] = token_logprobs_forward(logits, ids, top, ignore_index);
+        auto [logp, entropy, top_logp, top_ids, x2, id, stat] = token_logprobs_forward(logits, ids, top, ignore_index, false);
         return {logp, entropy, top_logp, top_ids};
     }
     const variable_list o = TokenLogprobs::apply(logits, ids, top, ignore_index);
@@ -299,17 +300,23 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, 
 std::vector<Tensor> grad_list(const py::object &parameters) {
     std::vector<Tensor> grads;
     auto add = [&](PyObject *o) {
+        if (Py_TYPE(o) == (PyTypeObject *)THPVariableClass) {
+            const Tensor &t = THPVariable_Unpack(o);
+            if (!t.requires_grad()) { grads.push_back(t); return; }
+        }
         TORCH_CHECK(THPVariable_Check(o), "parameters (leaves) or gradient tensors are wanted (got ", Py_TYPE(o)->tp_name, ")");
         const Tensor &t = THPVariable_Unpack(o);
-        if (Py_TYPE(o) == (PyTypeObject *)THPVariableClass && !t.requires_grad()) { grads.push_back(t); return; }
         TORCH_CHECK(t.requires_grad() || !ParameterClass || PyObject_IsInstance(o, ParameterClass) == 1,
                     "parameters (leaves) or gradient tensors are wanted (got ", Py_TYPE(o)->tp_name, " without a gradient)");
         TORCH_CHECK(t.is_leaf(), "parameters (leaves) or gradient tensors are wanted (got a tensor that an operation made and that requires a gradient)");
         if (t.grad().defined()) grads.push_back(t.grad());
     };
-    if (THPVariable_Check(parameters.ptr())) add(parameters.ptr());
-    else
-        for (const py::handle h : parameters) add(h.ptr());
+    if (THPVariable_Check(parameters.ptr())) { add(parameters.ptr()); return grads; }
+    const auto list = py::reinterpret_steal<py::object>(PySequence_Fast(parameters.ptr(), "parameters, gradient tensors or one of them are wanted"));
+    if (!list) throw py::error_already_set();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list.ptr());
+    grads.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) add(PySequence_Fast_GET_ITEM(list.ptr(), i));
     return grads;
 }
 

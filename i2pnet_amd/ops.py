@@ -1416,7 +1416,7 @@ class CBackend:
 
     def token_logprobs_forward(self, logits, ids, top, ignore_index):
         """logits [..., v], ids i64 [...] -> (logp [...], entropy [...], top_logp [..., top], top_ids [..., top], logits as rows, ids, stat)"""
-        return rows().token_logprobs_forward(logits, ids, top, ignore_index)
+        return rows().token_logprobs_forward(logits, ids, top, ignore_index, True)
 
     def token_logprobs_backward(self, x2, ids, ignore_index, stat, entropy, g_logp, g_entropy):
         """-> dlogits like x2"""

@@ -726,7 +726,7 @@ int i2p_rms_norm_bwd(long long rows, int d, int dtype, int wdtype, const void *s
                      long long ldgs, const void *w, const float *rstd, void *dx, void *dw, void *scratch, void *stream);
 /* Log probabilities of one given candidate per row of scores x [rows,v] (pitch ldx, v <= I2P_MAX_CANDIDATES), with the row's entropy and its `top` best alternatives
  * (0 <= top <= min(v, I2P_MAX_TOP); equal scores in index order): logp, entropy f32 [rows], top_logp f32 / top_ids i64 [rows,top];
- * stat f32 [rows,2] is for the backward.  ids i64 [rows]: a row with id == ignore is not read (logp = entropy = 0, top_logp = -inf,
+ * stat f32 [rows,2] (NULL: not wanted) is for the backward.  ids i64 [rows]: a row with id == ignore is not read (logp = entropy = 0, top_logp = -inf,
  * top_ids = -1, gradient 0); any other id outside [0, v) gives logp and gradient NaN.  A row of -inf: logp = -inf, entropy = 0, gradient 0;
  * NaN or +inf in a row: NaN.  scratch: i2p_token_logprobs_scratch(rows, v, dtype, top) bytes.
  * _bwd: g_logp, g_entropy f32 [rows] (either may be NULL = 0) -> dx [rows,v] (dense, of type dtype). */

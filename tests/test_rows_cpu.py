@@ -42,7 +42,7 @@ def test_rms_norm_backward_refusals(change):
 
 
 @pytest.mark.parametrize("change", [dict(rows=-1), dict(v=0), dict(v=(1 << 21) + 1, ldx=1 << 22), dict(dtype=3), dict(ldx=3), dict(top=-1), dict(top=9), dict(v=100, ldx=100, top=33),
-                                    dict(x=None), dict(ids=None), dict(logp=None), dict(entropy=None), dict(stat=None), dict(top_logp=None), dict(top_ids=None)])
+                                    dict(x=None), dict(ids=None), dict(logp=None), dict(entropy=None), dict(top_logp=None), dict(top_ids=None)])
 def test_token_logprobs_refusals(change):
     a = dict(rows=2, v=8, dtype=1, x=P, ldx=8, ids=P, ignore=-100, top=2, logp=P, entropy=P, stat=P, top_logp=P, top_ids=P, scratch=P) | change
     with pytest.raises(_lib.I2POpsError, match=BAD):

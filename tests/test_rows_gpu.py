@@ -782,7 +782,7 @@ def test_reads_and_writes_between_guards():
 
 @pytest.mark.parametrize("rows,v,dtype", [(2100, 16384, torch.bfloat16), (1100, 16388, torch.float32), (1100, 16389, torch.float32)])
 def test_token_logprobs_gradient_past_the_caches(rows, v, dtype):
-    """gradients of 64 MB and more, which are written past the caches where rows start on 16 bytes: the same bits as row by row"""
+    """gradients of 64 MB and more, which are written past the caches where rows start on 16 bytes"""
     x = torch.randn(rows, v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
     ids = torch.randint(0, v, (rows,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
     ids[5] = -100
@@ -791,12 +791,9 @@ def test_token_logprobs_gradient_past_the_caches(rows, v, dtype):
     o = loss.token_logprobs(leaf, ids)
     (d,) = torch.autograd.grad(o.logp.sum() + o.entropy.sum(), leaf)
     assert not d[5].any() and torch.isnan(d[rows - 1]).all()
-    for lo in range(0, rows - 1, 100):
-        part = x[lo:lo + 100].clone().requires_grad_(True)
-        q = loss.token_logprobs(part, ids[lo:lo + 100])
-        hi = min(lo + 100, rows - 1)
-        (e,) = torch.autograd.grad(q.logp.sum() + q.entropy.sum(), part)
-        # (another number of rows may cut them otherwise, and sum in another order)
-        n = hi - lo
-        diff = (d[lo:hi].float() - e[:n].float()).abs()
-        assert float((diff - (2 * half_step(dtype) + 1000 * U) * e[:n].float().abs()).max()) <= 1e-6
+    some = torch.tensor([0, 1, 2, 3, 4, 6, rows // 2, rows - 4, rows - 3, rows - 2])
+    one = torch.ones(len(some))
+    dx, mag = logp64(x[some.to(DEV)].cpu(), ids.cpu()[some], 0, one, one)[4:]
+    within(d[some.to(DEV)], dx, half_step(dtype) * dx.abs() + (8 * chain(v) + 2000) * U * mag + 1e-36, "dlogits")
+    # every row's gradient sums to 0 but for those errors; |dx| adds up to 2.2 over such a row and the terms' magnitudes to 20.5
+    assert float(d[6:rows - 1].double().sum(-1).abs().max()) < 40 * (half_step(dtype) + (8 * chain(v) + 2000) * U)
