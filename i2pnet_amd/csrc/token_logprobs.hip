@@ -97,7 +97,7 @@ template <int DT, int W, int E>
 __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W < 16) ? 6 : 8) void logprobs_fwd_kernel(FwdArgs a) {
     constexpr int T = 64 * W, VE = i2p_vec(DT), NV = E / VE;
     constexpr bool TINY = T * E == 512;
-    __shared__ float gmax[64], sums[2][W];
+    __shared__ float gmax[64], sums[2][W], bound;
     __shared__ skey list[LIST], best[W];
     __shared__ int count;
     const long long row = blockIdx.x / (unsigned)a.nsplit;      // (one row's slices stay together)
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
     const float m = lanes_max<64>(g), c = shift_of(m);
     // the largest value, to 16 bits of its order, that at least `top` groups reach
     float least = -__builtin_inff();
-    if (a.top) {
+    if (a.top && wave == 0) {                                   // (the others read it behind the next barrier)
         const unsigned o = order_of(g);
         unsigned b = 0u;
 #pragma unroll
@@ -152,6 +152,7 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
             if (__popcll(__ballot(o >= next)) >= a.top) b = next;
         }
         if (b > 0x007fffffu) least = value_of(b);               // (below: the order of -inf)
+        if (W > 1 && lane == 0) bound = least;
     }
     const Shift sh(c);
     float S = 0.f, U = 0.f;
@@ -192,6 +193,7 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
         else a.keys[(row * a.nsplit + part) * a.top + rank] = key;
     };
     if constexpr (W == 1) __syncthreads();                      // (`count`)
+    else least = bound;
     const bool plain = S == S;                                  // no NaN, no +inf
     unsigned long long bits = 0ull;                             // which of the thread's scores reach the bound
     if (plain && most >= least) {
