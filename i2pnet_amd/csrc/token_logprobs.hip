@@ -14,7 +14,8 @@
 // Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those (to 16 bits) is a value that at least k scores reach
 // and that few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow
 // that list and are searched k times instead.  10000 x 2000 fp32: 15.4 us without alternatives, 19.6 with 8, 24.8 with 32.
-// Backward: elementwise from the saved maximum, L and H; bound by reading the scores again and writing as much: 8192 x 131072 bf16 724 us, 5.9 TB/s.
+// Backward: elementwise from the saved maximum, L and H; bound by reading the scores again and writing as much: 8192 x 131072 bf16 725 us,
+// 5.9 TB/s.
 #include "rows_common.h"
 
 namespace {
