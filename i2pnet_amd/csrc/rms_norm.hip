@@ -31,7 +31,9 @@ template <int TPR, class Op> __device__ __forceinline__ unsigned row_reduce(unsi
     }
     return v;
 }
-template <int TPR> __device__ __forceinline__ float row_sum(float v, unsigned *red) { return __uint_as_float(row_reduce<TPR>(__float_as_uint(v), red, AddF{})); }
+template <int TPR> __device__ __forceinline__ float row_sum(float v, unsigned *red) {
+    return __uint_as_float(row_reduce<TPR>(__float_as_uint(v), red, AddF{}));
+}
 
 // the weights of a vector of columns (ones where there is no weight)
 template <int DT, bool TINY> __device__ __forceinline__ void ld_weight(const void *w, int wdtype, const Col<DT, TINY> &c, int d, float (&f)[i2p_vec(DT)]) {
@@ -347,7 +349,8 @@ inline long long bwd_blocks(long long rows, int d, int threads) {
 template <int DT, bool BWD, class F> bool by_width(int d, F f) {
     using std::integral_constant;
     const long long n = ((long long)d + i2p_vec(DT) - 1) / i2p_vec(DT);
-#define I2P_ROW(TPR, NV, TINY) { f(integral_constant<int, DT>{}, integral_constant<int, TPR>{}, integral_constant<int, NV>{}, std::bool_constant<TINY>{}); return true; }
+#define I2P_ROW(TPR, NV, TINY) \
+    { f(integral_constant<int, DT>{}, integral_constant<int, TPR>{}, integral_constant<int, NV>{}, std::bool_constant<TINY>{}); return true; }
     if (d < i2p_vec(DT)) I2P_ROW(8, 1, true)
     if (n <= 8) I2P_ROW(8, 1, false)
     if (n <= 16) I2P_ROW(16, 1, false)

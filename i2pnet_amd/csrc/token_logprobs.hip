@@ -86,7 +86,9 @@ __device__ __forceinline__ void skip_row(const FwdArgs &a, long long row) {
     for (int k = threadIdx.x; k < a.top; k += blockDim.x) { a.top_logp[row * a.top + k] = -__builtin_inff(); a.top_ids[row * a.top + k] = -1; }
 }
 
-template <int DT> __device__ __forceinline__ constexpr unsigned minus_inf() { return DT == I2P_F32 ? 0xff800000u : DT == I2P_BF16 ? 0xff80ff80u : 0xfc00fc00u; }
+template <int DT> __device__ __forceinline__ constexpr unsigned minus_inf() {
+    return DT == I2P_F32 ? 0xff800000u : DT == I2P_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+}
 
 // keeps the scores packed between the phases: the compiler would hold their fp32 values, and half as many waves would fit
 template <int N> __device__ __forceinline__ void hold(uint4 (&v)[N]) {
@@ -411,7 +413,8 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
         else if (slice <= 2048) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 32>), grid, dim3(64), 0, st, a);
         else if (slice <= 4096) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 16>), grid, dim3(256), 0, st, a);
         else if (slice <= SLICE) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 32>), grid, dim3(256), 0, st, a);
-        else if (DT != I2P_F32 && slice <= 2 * SLICE && (nsplit > 1 || rows > 512)) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, (DT == I2P_F32 ? 32 : 64)>), grid, dim3(256), 0, st, a);
+        else if (DT != I2P_F32 && slice <= 2 * SLICE && (nsplit > 1 || rows > 512))
+            hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, (DT == I2P_F32 ? 32 : 64)>), grid, dim3(256), 0, st, a);
         else if (slice <= 16384) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 16, 16>), grid, dim3(1024), 0, st, a);
         else hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 16, 32>), grid, dim3(1024), 0, st, a);
         if (nsplit > 1) hipLaunchKernelGGL(logprobs_join_kernel, dim3((unsigned)k), dim3(JT), 0, st, a, dtype);
@@ -434,9 +437,11 @@ extern "C" int i2p_token_logprobs_bwd(long long rows, int v, int dtype, const vo
         const int nvec = (v + i2p_vec(DT) - 1) / i2p_vec(DT);
         auto go = [&](auto tpr) {
             constexpr int TPR = tpr.value;
-            const BwdArgs a{rows, v, (const char *)x, ldx, ids, ignore, stat, entropy, g_logp, g_entropy, (char *)dx, stream_out, (nvec + TPR * BV - 1) / (TPR * BV)};
+            const BwdArgs a{rows, v, (const char *)x, ldx, ids, ignore, stat, entropy, g_logp, g_entropy, (char *)dx, stream_out,
+                            (nvec + TPR * BV - 1) / (TPR * BV)};
             const long long blocks = (rows * a.pieces + 256 / TPR - 1) / (256 / TPR);
-            hipLaunchKernelGGL((logprobs_bwd_kernel<DT, TPR>), dim3((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22))), dim3(256), 0, (hipStream_t)stream, a);
+            hipLaunchKernelGGL((logprobs_bwd_kernel<DT, TPR>), dim3((unsigned)(blocks < (1 << 22) ? blocks : (1 << 22))), dim3(256), 0,
+                               (hipStream_t)stream, a);
         };
         if (nvec <= 16 * BV) go(std::integral_constant<int, 16>{});
         else if (nvec <= 64 * BV) go(std::integral_constant<int, 64>{});
