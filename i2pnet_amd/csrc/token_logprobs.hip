@@ -6,7 +6,7 @@
 // The maximum and L are kept apart for the backward pass: rounded into one number, scores of a few hundred would lose the digits of L.
 // A row without candidates (all -inf): logp -inf, H 0, gradient 0.  +inf or NaN in a row: logp, H, top_logp and the gradient are NaN.
 //
-// Forward: reads the scores once.  A row, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at most 32 scores a
+// Forward: reads the scores once.  A row of more than 128 scores, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at most 32 scores a
 // thread, 64 of the 16-bit types), so that the maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k
 // best in the workspace and a second launch joins them.  8192 x 131072 bf16: 455 us, 4.7 TB/s (a plain sum of that much reads 4.0 TB/s here);
 // the vector units are 80 % busy beside it, some 8 instructions a score (PMC on slices of 8192: 413 a wave of 32 scores a lane).  4096 x 32000:
@@ -99,7 +99,6 @@ template <int N> __device__ __forceinline__ void hold(uint4 (&v)[N]) {
 template <int DT, int W, int E>
 __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W < 16) ? 6 : 8) void logprobs_fwd_kernel(FwdArgs a) {
     constexpr int T = 64 * W, VE = i2p_vec(DT), NV = E / VE;
-    constexpr bool TINY = T * E == 512;
     __shared__ float gmax[64], sums[2][W], bound;
     __shared__ skey list[LIST], best[W];
     __shared__ int count;
@@ -112,9 +111,9 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
     uint4 v[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const Col<DT, TINY> c(j * T + t, n);
+        const Col<DT> c(j * T + t, n);
         v[j] = c.load(x, n, minus_inf<DT>());
-        if (c.skip || (TINY && c.in && c.at + VE > n)) {        // what is not this vector's reads as -inf
+        if (c.skip) {                                           // what is not this vector's reads as -inf
             float f[VE];
             unpack<DT>(v[j], f);
 #pragma unroll
@@ -203,7 +202,7 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             if (!(vmax[j] >= least)) continue;
-            const Col<DT, TINY> col(j * T + t, n);
+            const Col<DT> col(j * T + t, n);
             float f[VE];
             unpack<DT>(v[j], f);
 #pragma unroll
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
         if (bits) {
             const int i = __ffsll(bits) - 1, at = base + __popcll(has & ((1ull << lane) - 1ull));
             bits &= bits - 1ull;
-            const int col = Col<DT, TINY>(i / VE * T + t, n).at + i % VE;
+            const int col = Col<DT>(i / VE * T + t, n).at + i % VE;
             if (at < LIST) list[at] = key_of(ld1<DT>(x, col), (unsigned)(lo + col));
         }
     }
@@ -252,6 +251,63 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
         __syncthreads();
         if (t == 0) put(k, top);
         last = top;
+    }
+}
+
+// Rows of at most 128 scores: 16 lanes share one (8 scores each, lane by lane), so that a wave has four.  The alternatives are searched one
+// after the other.  60000 x 32 fp32: 21 us with a wave per row, 5.2 here (41 and 12.4 with 3 alternatives)
+constexpr int SMALL = 128;
+__device__ __forceinline__ skey row16_best(skey k) {
+    auto step = [&](unsigned lo, unsigned hi) { const skey u = ((skey)hi << 32) | lo; k = u > k ? u : k; };
+    step(i2p_dpp_u32<0xB1>((unsigned)k), i2p_dpp_u32<0xB1>((unsigned)(k >> 32)));
+    step(i2p_dpp_u32<0x4E>((unsigned)k), i2p_dpp_u32<0x4E>((unsigned)(k >> 32)));
+    step(i2p_dpp_u32<0x141>((unsigned)k), i2p_dpp_u32<0x141>((unsigned)(k >> 32)));
+    step(i2p_dpp_u32<0x140>((unsigned)k), i2p_dpp_u32<0x140>((unsigned)(k >> 32)));
+    return k;
+}
+
+template <int DT> __global__ __launch_bounds__(256) void logprobs_small_kernel(FwdArgs a) {
+    constexpr int E = SMALL / 16;
+    const long long row = (long long)blockIdx.x * 16 + threadIdx.x / 16;
+    if (row >= a.rows) return;                                  // (16 lanes leave together: the reductions below stay among 16)
+    const int t = threadIdx.x % 16;
+    const long long id = a.ids[row];
+    const char *x = a.x + row * a.ldx * i2p_esize(DT);
+    if (id == a.ignore) {
+        if (t == 0) { a.logp[row] = 0.f; a.entropy[row] = 0.f; if (a.stat) a.stat[2 * row] = a.stat[2 * row + 1] = 0.f; }
+        for (int k = t; k < a.top; k += 16) { a.top_logp[row * a.top + k] = -__builtin_inff(); a.top_ids[row * a.top + k] = -1; }
+        return;
+    }
+    float f[E], m = -__builtin_inff();
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int i = e * 16 + t;
+        f[e] = i < a.v ? ld1<DT>(x, i) : -__builtin_inff();
+        m = fmaxf(m, f[e]);
+    }
+    const float xid = t == 0 && id >= 0 && id < a.v ? ld1<DT>(x, id) : 0.f;
+    const float c = shift_of(lanes_max<16>(m));
+    float S = 0.f, U = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (e * 16 < a.v) {
+            const float y = (f[e] - c) * LOG2E, p = __builtin_amdgcn_exp2f(y);
+            S += p;
+            U = __builtin_fmaf(fmaxf(y, -300.f), p, U);
+        }
+    S = lanes_sum<16>(S);
+    U = LN2 * lanes_sum<16>(U);
+    if (t == 0) finish_row(a, row, id, xid, c, S, U);
+    skey last = ~0ull;
+    for (int k = 0; k < a.top; ++k) {
+        skey best = 0ull;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const skey key = e * 16 + t < a.v ? key_of(f[e], (unsigned)(e * 16 + t)) : 0ull;
+            if (key < last && key > best) best = key;
+        }
+        last = row16_best(best);
+        if (t == 0) put_top(a, row, k, last, c, S);
     }
 }
 
@@ -401,7 +457,7 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
     cut(rows, v, dtype, nsplit, slice);
     if (nsplit > 1 && (!scratch || ((uintptr_t)scratch & 15))) return I2P_ERR_BAD_ARG;
     hipStream_t st = (hipStream_t)stream;
-    const long long most = (1 << 21) / nsplit;                  // rows of a launch: a grid has fewer than 2^32 threads
+    const long long most = (1 << 21) / nsplit;          // rows of a launch: a grid has fewer than 2^32 threads
     for (long long r = 0; r < rows; r += most) by_type(dtype, [&](auto dt) {
         const long long k = rows - r < most ? rows - r : most;
         const FwdArgs a{k, v, (const char *)x + r * ldx * i2p_esize(dtype), ldx, ids + r, ignore, top, logp + r, entropy + r, stat ? stat + 2 * r : nullptr,
@@ -409,7 +465,8 @@ extern "C" int i2p_token_logprobs_fwd(long long rows, int v, int dtype, const vo
                         (skey *)((char *)scratch + rows * nsplit * 16) + r * nsplit * top};
         const dim3 grid((unsigned)(k * nsplit));
         constexpr int DT = dt.value;
-        if (slice <= 512) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 8>), grid, dim3(64), 0, st, a);
+        if (v <= SMALL) hipLaunchKernelGGL((logprobs_small_kernel<DT>), dim3((unsigned)((k + 15) / 16)), dim3(256), 0, st, a);
+        else if (slice <= 512) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 8>), grid, dim3(64), 0, st, a);
         else if (slice <= 2048) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 1, 32>), grid, dim3(64), 0, st, a);
         else if (slice <= 4096) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 16>), grid, dim3(256), 0, st, a);
         else if (slice <= SLICE) hipLaunchKernelGGL((logprobs_fwd_kernel<DT, 4, 32>), grid, dim3(256), 0, st, a);
