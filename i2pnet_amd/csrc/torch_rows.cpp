@@ -71,12 +71,21 @@ int type_of(const Tensor &t) {
 
 void *ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
 
+// A forward-mode tangent would be lost without a word: the outputs come from the kernels and carry none
+void primal(const Tensor &t, const char *what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, " has a forward-mode tangent: the row operators have no forward-mode derivative");
+}
+void primal(const OptTensor &t, const char *what) {
+    if (t) primal(*t, what);
+}
+
 // a tensor [..., d] as rows of pitch ld; a copy only where the columns are not next to each other or rows overlap
 struct Rows {
     Tensor t;
     int64_t n, d, ld;
     int type;
     Rows(const Tensor &x, const char *what, const Tensor *like = nullptr) {
+        primal(x, what);
         TORCH_CHECK(x.is_cuda(), what, " must be a cuda tensor (got ", x.device(), ")");
         type = type_of(x);
         TORCH_CHECK(type >= 0, what, " must be float32, bfloat16 or float16 (got ", x.scalar_type(), ")");
@@ -123,6 +132,8 @@ int weight_type(const OptTensor &w, const Tensor &x, int64_t d) {
 
 // -> y, the stream (x itself, as rows, without a residual), rstd (undefined unless wanted)
 std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, bool want_rstd) {
+    primal(residual, "residual");
+    primal(weight, "weight");
     const Rows a(x, "x");
     std::optional<Rows> r;
     if (residual) r.emplace(*residual, "residual", &x);
@@ -139,6 +150,8 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor &x, const OptTe
 std::tuple<Tensor, Tensor, OptTensor> rms_norm_q8(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, int64_t group) {
     TORCH_CHECK(!at::GradMode::is_enabled() || !(x.requires_grad() || (weight && weight->requires_grad()) || (residual && residual->requires_grad())),
                 "rms_norm_q8 has no gradient: call it under torch.no_grad() or on detached tensors");
+    primal(residual, "residual");
+    primal(weight, "weight");
     TORCH_CHECK_VALUE(group == 0 || (group >= 32 && group <= 512 && (group & (group - 1)) == 0),
                       "rms_norm_q8: group must be 0 (the whole row) or a power of two from 32 to 512 (got ", group, ")");
     const Rows a(x, "x");
@@ -160,6 +173,8 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_q8(const Tensor &x, const OptTens
 // gs: the stream's gradient or none; s may be given as rows -> dx like gy, dw like weight
 std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor &s, const OptTensor &weight, const Tensor &rstd, const Tensor &gy, const OptTensor &gs,
                                                 bool need_dw) {
+    primal(s, "s");
+    primal(gs, "gs");
     const Rows g(gy, "gy"), a(s, "s");
     TORCH_CHECK(a.n == g.n && a.d == g.d && a.type == g.type && s.device() == gy.device(), "gy must be ", s.scalar_type(), " with the rows of s");
     std::optional<Rows> e;
@@ -250,6 +265,8 @@ Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t
 // x2, ids, stat, entropy as the forward left them -> the gradient, dense, like x2
 Tensor token_logprobs_backward(const Tensor &x2, const Tensor &ids, int64_t ignore_index, const Tensor &stat, const Tensor &entropy, const OptTensor &g_logp,
                                const OptTensor &g_entropy) {
+    primal(g_logp, "g_logp");
+    primal(g_entropy, "g_entropy");
     const Rows a(x2, "logits");
     auto dense = [&](const OptTensor &g, const char *what) -> OptTensor {
         if (!g) return std::nullopt;
@@ -323,6 +340,7 @@ std::vector<Tensor> grad_list(const py::object &parameters) {
 // total norm f32 0-d of a list that is not empty; no max_norm: nothing is clipped
 Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optional<double> max_norm, const OptTensor &out) {
     TORCH_CHECK(!grads.empty(), "clip_grad_norm: no gradients");
+    primal(out, "out");
     const auto device = grads[0].device();
     const int n = (int)grads.size();
     std::vector<const void *> ptrs(n);
@@ -331,6 +349,7 @@ Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optio
     long long total = 0;
     for (int i = 0; i < n; ++i) {
         const Tensor &g = grads[i];
+        primal(g, "a gradient");
         types[i] = type_of(g);
         TORCH_CHECK(types[i] >= 0, "gradients must be float32, bfloat16 or float16 (got ", g.scalar_type(), ")");
         TORCH_CHECK(g.is_cuda() && g.device() == device, "gradients must be cuda tensors on one device (got ", g.device(), ")");

@@ -69,5 +69,6 @@ def token_logprobs(logits, ids, top=0, ignore_index=-100):
     ids: int64.  A row whose id is `ignore_index` is padding: it is not read, logp and entropy are 0, its alternatives -1 with -inf, its
     gradient 0.  Any other id outside [0, v) makes that row's logp and gradient NaN (ids are not read on the host).  A row without
     candidates (all -inf) has logp -inf, entropy 0 and gradient 0; a NaN or +inf makes the row's results NaN.
-    top: 0 .. min(v, 32); equal scores are listed by index.  logp and entropy are differentiable in logits, once; the alternatives are not."""
+    top: 0 .. min(v, 32); equal scores are listed by index.  logp and entropy are differentiable in logits, once, in reverse
+    mode; the alternatives are not."""
     return TokenLogprobs(*ops.rows().token_logprobs(logits, ids, top, ignore_index))

@@ -688,7 +688,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
     layers a row's result does not depend on the other rows, and `_unit_variance` is the reference's form of it without a weight.
 
     x, residual: [..., d] float32, bfloat16 or float16 of any d and row pitch (rows without unit column stride are copied first);
-    weight: [d], float32 or x's type, None = ones.  Differentiable in x, residual and weight, once."""
+    weight: [d], float32 or x's type, None = ones.  Differentiable in x, residual and weight, once, in reverse mode (forward-mode
+    tangents are refused)."""
     r = ops.rows()
     return r.rms_norm(x, weight, eps) if residual is None else r.rms_norm_residual(x, weight, residual, eps)
 

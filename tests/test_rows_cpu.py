@@ -146,3 +146,38 @@ def test_lists_of_parameters():
     assert train._grad_list([a, b, c, raw])[0] is a.grad and len(train._grad_list([a, b, c, raw])) == 2
     assert train._grad_list(raw)[0] is raw and train._grad_list(x for x in ()) == []
     assert isinstance(ops.MAX_TOP, int)
+
+
+def rows_calls(x, r, w, ids):
+    """every public row operator on the given tensors"""
+    return {"rms_norm": lambda: modules.rms_norm(x, w), "rms_norm residual": lambda: modules.rms_norm(x, w, residual=r)[0],
+            "rms_norm_q8": lambda: modules.rms_norm_q8(x, w, residual=r)[0], "token_logprobs": lambda: loss.token_logprobs(x, ids).logp,
+            "grad_norm": lambda: train.grad_norm([x]), "clip_grad_norm_": lambda: train.clip_grad_norm_([x], 1.0),
+            "clip_grad_norm_ out": lambda: train.clip_grad_norm_([x], 1.0, out=r.reshape(-1))}
+
+
+@pytest.mark.parametrize("name", sorted(rows_calls(*[torch.zeros(1)] * 4)))
+@pytest.mark.parametrize("which", ["x", "r", "w"])
+def test_forward_mode_is_refused(name, which):
+    """a tangent would be lost without a word: the outputs carry none"""
+    t = {"x": torch.ones(2, 8), "r": torch.ones(2, 8), "w": torch.ones(8)}
+    with torch.autograd.forward_ad.dual_level():
+        t[which] = torch.autograd.forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        uses = {"x": True, "r": name in ("rms_norm residual", "rms_norm_q8", "clip_grad_norm_ out"),
+                "w": name.startswith("rms_norm")}[which]
+        if uses:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                rows_calls(t["x"], t["r"], t["w"], torch.zeros(2, dtype=torch.long))[name]()
+
+
+def test_forward_mode_through_a_backward_pass_is_refused():
+    s, g, one = torch.ones(2, 8), torch.ones(2, 8), torch.ones(2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual
+        for a, b, c in ((dual(s, g), g, None), (s, dual(g, g), None), (s, g, dual(g, g))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.rows().rms_norm_backward(a, None, one, b, c, False)
+        ids, stat = torch.zeros(2, dtype=torch.long), torch.zeros(2, 2)
+        for a, b, c in ((dual(s, g), one, one), (s, dual(one, one), None), (s, None, dual(one, one))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.rows().token_logprobs_backward(a, ids, -100, stat, one, b, c)
