@@ -4,12 +4,15 @@
 //
 // Why not Python over ctypes, as for the other operators: these calls are short (2 .. 20 us on the device).  A backward pass in Python costs
 // about 90 us for the hand-over of the interpreter to autograd's device thread alone, and a list of 254 gradients 100 us of attribute reads.
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 
@@ -70,6 +73,15 @@ int type_of(const Tensor &t) {
 }
 
 void *ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
+
+// The kernels are launched by address, which nothing that records torch's operators sees: a trace would hold the allocation of the outputs
+// alone and return what memory held when it is replayed
+void eager(const char *name) {
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() &&
+                    !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
+                name, " cannot be traced (torch.jit.trace, make_fx, torch.export): the trace would not hold its kernels");
+}
 
 // A forward-mode tangent would be lost without a word: the outputs come from the kernels and carry none
 void primal(const Tensor &t, const char *what) {
@@ -132,6 +144,7 @@ int weight_type(const OptTensor &w, const Tensor &x, int64_t d) {
 
 // -> y, the stream (x itself, as rows, without a residual), rstd (undefined unless wanted)
 std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, bool want_rstd) {
+    eager("rms_norm");
     primal(residual, "residual");
     primal(weight, "weight");
     const Rows a(x, "x");
@@ -148,6 +161,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor &x, const OptTe
 }
 
 std::tuple<Tensor, Tensor, OptTensor> rms_norm_q8(const Tensor &x, const OptTensor &weight, const OptTensor &residual, double eps, int64_t group) {
+    eager("rms_norm_q8");
     TORCH_CHECK(!at::GradMode::is_enabled() || !(x.requires_grad() || (weight && weight->requires_grad()) || (residual && residual->requires_grad())),
                 "rms_norm_q8 has no gradient: call it under torch.no_grad() or on detached tensors");
     primal(residual, "residual");
@@ -173,6 +187,7 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_q8(const Tensor &x, const OptTens
 // gs: the stream's gradient or none; s may be given as rows -> dx like gy, dw like weight
 std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor &s, const OptTensor &weight, const Tensor &rstd, const Tensor &gy, const OptTensor &gs,
                                                 bool need_dw) {
+    eager("rms_norm");
     primal(s, "s");
     primal(gs, "gs");
     const Rows g(gy, "gy"), a(s, "s");
@@ -238,6 +253,7 @@ std::tuple<Tensor, Tensor> rms_norm_residual(const Tensor &x, const OptTensor &w
 // -> logp, entropy, top_logp, top_ids, the scores as rows, ids (contiguous), stat
 using Logprobs = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t top, int64_t ignore_index, bool want_stat) {
+    eager("token_logprobs");
     const Rows a(logits, "logits");
     TORCH_CHECK(ids.scalar_type() == at::kLong && ids.device() == logits.device() && ids.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                 "ids must be int64 ", logits.sizes().slice(0, logits.dim() - 1), " on ", logits.device(), " (got ", ids.scalar_type(), " ", ids.sizes(),
@@ -265,6 +281,7 @@ Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t
 // x2, ids, stat, entropy as the forward left them -> the gradient, dense, like x2
 Tensor token_logprobs_backward(const Tensor &x2, const Tensor &ids, int64_t ignore_index, const Tensor &stat, const Tensor &entropy, const OptTensor &g_logp,
                                const OptTensor &g_entropy) {
+    eager("token_logprobs");
     primal(g_logp, "g_logp");
     primal(g_entropy, "g_entropy");
     const Rows a(x2, "logits");
@@ -339,6 +356,7 @@ std::vector<Tensor> grad_list(const py::object &parameters) {
 
 // total norm f32 0-d of a list that is not empty; no max_norm: nothing is clipped
 Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optional<double> max_norm, const OptTensor &out) {
+    eager("clip_grad_norm");
     TORCH_CHECK(!grads.empty(), "clip_grad_norm: no gradients");
     primal(out, "out");
     const auto device = grads[0].device();

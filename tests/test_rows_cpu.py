@@ -181,3 +181,27 @@ def test_forward_mode_through_a_backward_pass_is_refused():
         for a, b, c in ((dual(s, g), one, one), (s, dual(one, one), None), (s, None, dual(one, one))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 ops.rows().token_logprobs_backward(a, ids, -100, stat, one, b, c)
+
+
+@pytest.mark.parametrize("name", sorted(rows_calls(*[torch.zeros(1)] * 4)))
+def test_a_call_that_is_being_traced_is_refused(name):
+    """a trace would hold the allocation of the outputs and not the launch: replayed, it would return what memory held"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, r, w, ids = torch.ones(2, 8), torch.ones(2, 8), torch.ones(8), torch.zeros(2, dtype=torch.long)
+    f = lambda a, b, c: rows_calls(a, b, c, ids)[name]() + 0
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(f, (x, r, w), check_trace=False)
+    for pre in (False, True):
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f, pre_dispatch=pre)(x, r, w)
+
+
+def test_a_backward_pass_that_is_being_traced_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    s, one, ids = torch.ones(2, 8), torch.ones(2), torch.zeros(2, dtype=torch.long)
+    for f in (lambda a: ops.rows().rms_norm_backward(a, None, one, a, None, False)[0],
+              lambda a: ops.rows().token_logprobs_backward(a, ids, -100, torch.zeros(2, 2), one, one, None)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (s,), check_trace=False)
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f)(s)
