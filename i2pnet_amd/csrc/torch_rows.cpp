@@ -91,6 +91,10 @@ void primal(const OptTensor &t, const char *what) {
     if (t) primal(*t, what);
 }
 
+// the values that a tensor stands for, in memory: torch may keep a sign beside it as a flag (the imaginary part of a conjugate)
+Tensor plain(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+OptTensor plain(const OptTensor &t) { return t ? OptTensor(plain(*t)) : std::nullopt; }
+
 // a tensor [..., d] as rows of pitch ld; a copy only where the columns are not next to each other or rows overlap
 struct Rows {
     Tensor t;
@@ -110,9 +114,9 @@ struct Rows {
         TORCH_CHECK(d <= I2P_MAX_ROW, what, ": rows of ", d, " elements are too long");
         n = x.numel() / d;
         ld = d;
-        t = x;
-        if (x.is_contiguous()) return;
-        if (x.dim() != 2) t = x.reshape({n, d});
+        t = plain(x);
+        if (t.is_contiguous()) return;
+        if (x.dim() != 2) t = t.reshape({n, d});
         if ((d > 1 && t.stride(1) != 1) || (n > 1 && t.stride(0) < d)) t = t.contiguous();
         if (n > 1) ld = t.stride(0);
     }
@@ -151,10 +155,11 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor &x, const OptTe
     std::optional<Rows> r;
     if (residual) r.emplace(*residual, "residual", &x);
     const int wt = weight_type(weight, x, a.d);
+    const OptTensor w = plain(weight);
     Tensor y = at::empty(x.sizes(), x.options()), s = r ? at::empty(x.sizes(), x.options()) : a.t, rstd;
     if (want_rstd) rstd = at::empty({a.n}, x.options().dtype(at::kFloat));
     const On on(x.device());
-    check(abi.rms_norm_fwd(a.n, (int)a.d, a.type, wt, a.t.data_ptr(), a.ld, r ? r->t.data_ptr() : nullptr, r ? r->ld : 0, ptr(weight), (float)eps,
+    check(abi.rms_norm_fwd(a.n, (int)a.d, a.type, wt, a.t.data_ptr(), a.ld, r ? r->t.data_ptr() : nullptr, r ? r->ld : 0, ptr(w), (float)eps,
                            r ? s.data_ptr() : nullptr, y.data_ptr(), want_rstd ? rstd.data_ptr<float>() : nullptr, on.stream()),
           "i2p_rms_norm_fwd");
     return {y, s, rstd};
@@ -172,13 +177,14 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_q8(const Tensor &x, const OptTens
     std::optional<Rows> r;
     if (residual) r.emplace(*residual, "residual", &x);
     const int wt = weight_type(weight, x, a.d);
+    const OptTensor w = plain(weight);
     std::vector<int64_t> groups = x.sizes().vec();
     groups.back() = group ? (a.d + group - 1) / group : 1;
     Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(groups, x.options().dtype(at::kFloat));
     OptTensor s;
     if (r) s = at::empty(x.sizes(), x.options());
     const On on(x.device());
-    check(abi.rms_norm_q8(a.n, (int)a.d, a.type, wt, a.t.data_ptr(), a.ld, r ? r->t.data_ptr() : nullptr, r ? r->ld : 0, ptr(weight), (float)eps,
+    check(abi.rms_norm_q8(a.n, (int)a.d, a.type, wt, a.t.data_ptr(), a.ld, r ? r->t.data_ptr() : nullptr, r ? r->ld : 0, ptr(w), (float)eps,
                           (int)group, ptr(s), (unsigned char *)q.data_ptr(), scale.data_ptr<float>(), on.stream()),
           "i2p_rms_norm_q8");
     return {q, scale, s};
@@ -195,15 +201,16 @@ std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor &s, const OptTensor
     std::optional<Rows> e;
     if (gs) e.emplace(*gs, "gs", &gy);
     const int wt = weight_type(weight, s, a.d);
+    const OptTensor w = plain(weight);
     TORCH_CHECK(rstd.is_contiguous() && rstd.scalar_type() == at::kFloat && rstd.numel() == a.n && rstd.device() == s.device(), "rstd must be float32 [", a.n, "]");
     Tensor dx = at::empty(gy.sizes(), gy.options());
     OptTensor dw, scratch;
     TORCH_CHECK(!need_dw || weight, "rms_norm_backward: the weight's gradient is wanted, but there is no weight");
-    if (need_dw) dw = a.n ? at::empty_like(*weight) : at::zeros_like(*weight);
+    if (need_dw) dw = a.n ? at::empty(weight->sizes(), weight->options()) : at::zeros(weight->sizes(), weight->options());
     if (a.n == 0) return {dx, dw};
     if (need_dw) scratch = at::empty({abi.rms_norm_bwd_scratch(a.n, (int)a.d)}, gy.options().dtype(at::kByte));
     const On on(gy.device());
-    check(abi.rms_norm_bwd(a.n, (int)a.d, a.type, wt, a.t.data_ptr(), a.ld, g.t.data_ptr(), g.ld, e ? e->t.data_ptr() : nullptr, e ? e->ld : 0, ptr(weight),
+    check(abi.rms_norm_bwd(a.n, (int)a.d, a.type, wt, a.t.data_ptr(), a.ld, g.t.data_ptr(), g.ld, e ? e->t.data_ptr() : nullptr, e ? e->ld : 0, ptr(w),
                            rstd.data_ptr<float>(), dx.data_ptr(), ptr(dw), ptr(scratch), on.stream()),
           "i2p_rms_norm_bwd");
     return {dx, dw};
@@ -261,7 +268,7 @@ Logprobs token_logprobs_forward(const Tensor &logits, const Tensor &ids, int64_t
     TORCH_CHECK_VALUE(a.d <= I2P_MAX_CANDIDATES, "token_logprobs: rows of at most ", I2P_MAX_CANDIDATES, " candidates (got ", a.d, ")");
     TORCH_CHECK_VALUE(top >= 0 && top <= a.d && top <= I2P_MAX_TOP, "token_logprobs: top must be between 0 and ", std::min<int64_t>(a.d, I2P_MAX_TOP),
                       " (got ", top, ")");
-    const Tensor id = ids.contiguous();
+    const Tensor id = plain(ids).contiguous();
     const auto f32 = logits.options().dtype(at::kFloat);
     std::vector<int64_t> list = ids.sizes().vec();
     list.push_back(top);
@@ -288,7 +295,7 @@ Tensor token_logprobs_backward(const Tensor &x2, const Tensor &ids, int64_t igno
     auto dense = [&](const OptTensor &g, const char *what) -> OptTensor {
         if (!g) return std::nullopt;
         TORCH_CHECK(g->scalar_type() == at::kFloat && g->device() == x2.device() && g->numel() == a.n, what, " must be float32 with ", a.n, " elements");
-        return g->contiguous();
+        return plain(*g).contiguous();
     };
     TORCH_CHECK(ids.is_contiguous() && ids.numel() == a.n && stat.is_contiguous() && stat.numel() == 2 * a.n && entropy.is_contiguous() &&
                     entropy.numel() == a.n, "token_logprobs: ids, stat and entropy must be the forward's");
@@ -364,6 +371,7 @@ Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optio
     std::vector<const void *> ptrs(n);
     std::vector<long long> sizes(n);
     std::vector<int> types(n);
+    std::vector<Tensor> copies;                 // (in place a flagged sign changes nothing: what is scaled is its negative)
     long long total = 0;
     for (int i = 0; i < n; ++i) {
         const Tensor &g = grads[i];
@@ -373,12 +381,13 @@ Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optio
         TORCH_CHECK(g.is_cuda() && g.device() == device, "gradients must be cuda tensors on one device (got ", g.device(), ")");
         TORCH_CHECK(g.layout() == at::kStrided && g.is_non_overlapping_and_dense(), "gradients must be dense (got sizes ", g.sizes(), ", strides ",
                     g.layout() == at::kStrided ? g.strides() : at::IntArrayRef(), ")");
-        ptrs[i] = g.data_ptr();
+        if (out && g.is_neg()) copies.push_back(g.resolve_neg());
+        ptrs[i] = out && g.is_neg() ? copies.back().data_ptr() : g.data_ptr();
         total += sizes[i] = g.numel();
     }
     if (out)
         TORCH_CHECK(out->device() == device && out->scalar_type() == at::kFloat && out->dim() == 1 && out->is_contiguous() && out->numel() == total &&
-                        !(out->requires_grad() && out->is_leaf()),
+                        !out->is_neg() && !(out->requires_grad() && out->is_leaf()),
                     "out must be a contiguous float32 [", total, "] on ", device, " (got ", out->scalar_type(), " ", out->sizes(), " on ", out->device(), ")");
     const auto f32 = grads[0].options().dtype(at::kFloat).memory_format(std::nullopt);
     const Tensor scratch = at::empty({abi.grad_norm_scratch(n, sizes.data())}, f32.dtype(at::kByte)), norm = at::empty({}, f32);

@@ -797,3 +797,34 @@ def test_token_logprobs_gradient_past_the_caches(rows, v, dtype):
     within(d[some.to(DEV)], dx, half_step(dtype) * dx.abs() + (8 * chain(v) + 2000) * U * mag + 1e-36, "dlogits")
     # every row's gradient sums to 0 but for those errors; |dx| adds up to 2.2 over such a row and the terms' magnitudes to 20.5
     assert float(d[6:rows - 1].double().sum(-1).abs().max()) < 40 * (half_step(dtype) + (8 * chain(v) + 2000) * U)
+
+
+def test_negated_views():
+    """views whose sign is a flag that torch keeps beside them (the imaginary part of a conjugate) stand for the negated memory"""
+    for d in (1, 40):
+        z = torch.complex(rnd(6, d, seed=1), rnd(6, d, seed=2)).to(DEV)
+        flat = rnd(6, d, seed=3).to(DEV)
+        for a in (z.conj().imag, torch._neg_view(flat)):
+            assert a.is_neg()
+            b = a.clone(memory_format=torch.contiguous_format).resolve_neg().clone()
+            b.copy_(-(z.imag if a.stride() != flat.stride() else flat))
+            w, gy, one = torch._neg_view(rnd(d, seed=4).to(DEV)), torch._neg_view(rnd(6, d, seed=5).to(DEV)), torch._neg_view(rnd(6, seed=6).to(DEV))
+            ids = torch._neg_view(-torch.tensor([0] * 5 + [d - 1], device=DEV))
+            sides = []
+            for x, real in ((a, lambda t: t), (b, lambda t: 0 + t)):
+                x, p = x.detach().requires_grad_(True), real(w).detach().requires_grad_(True)
+                y, s = modules.rms_norm(x, p, residual=x)
+                alone = modules.rms_norm(x, p)
+                o = loss.token_logprobs(x, real(ids), top=1)
+                q = modules.rms_norm_q8(x.detach(), p.detach(), residual=x.detach(), group=32)
+                gx, gp = torch.autograd.grad([y, s], [x, p], [real(gy), real(gy)])
+                (gl,) = torch.autograd.grad([o.logp, o.entropy], [x], [real(one), real(one)])
+                out = torch.empty(6 * d, device=DEV)
+                n = train.clip_grad_norm_([real(gy)], 0.5, out=out)
+                sides.append([y, s, alone, gx, gp, gl, out, n, *o, q[0].view(torch.uint8), *q[1:]])
+            for i, (p, q) in enumerate(zip(*sides)):
+                assert torch.equal(p, q), (d, i)
+    base = torch.full((4,), -3.0, device=DEV)
+    assert float(train.clip_grad_norm_([torch._neg_view(base)], 3.0)) == 6.0 and float((base + 1.5).abs().max()) < 1e-6
+    with pytest.raises(RuntimeError, match="out must"):
+        train.clip_grad_norm_([base], 1.0, out=torch._neg_view(torch.empty(4, device=DEV)))
