@@ -828,3 +828,19 @@ def test_negated_views():
     assert float(train.clip_grad_norm_([torch._neg_view(base)], 3.0)) == 6.0 and float((base + 1.5).abs().max()) < 1e-6
     with pytest.raises(RuntimeError, match="out must"):
         train.clip_grad_norm_([base], 1.0, out=torch._neg_view(torch.empty(4, device=DEV)))
+
+
+@pytest.mark.parametrize("count", [1800, 2048])
+def test_the_norm_does_not_depend_on_the_call(count):
+    """squares whose sum lies a few last places of fp64 above a tie of fp32: the order of the additions shows in the rounded norm.  2^24, 4096,
+    4096 and 1 have (2^24 + 1)^2 as their sum; 0.15^2 = 0.0225 is lost beside it alone (half a last place: 2^-5) and kept in pairs"""
+    vals = torch.zeros(count)
+    vals[0], vals[1], vals[2], vals[3] = 2.0 ** 24, 4096.0, 4096.0, 1.0
+    vals[256::256] = 0.15
+    gs = [vals[i:i + 1].to(DEV) for i in range(count)]
+    n = train.grad_norm(gs)
+    out = torch.empty(count, device=DEV)
+    for limit in (1e9, 1.0):
+        assert torch.equal(train.clip_grad_norm_(gs, limit, out=out), n)
+    assert torch.equal(train.clip_grad_norm_([g.clone() for g in gs], 1e9), n)
+    assert abs(float(n) - 16777217.0) <= 1.0
