@@ -5,9 +5,11 @@
 //   8 bits: scale = max |s rstd w| / 448 over a group of columns (1 where that is below the smallest normal number), q = e4m3(s rstd w / scale)
 //   backward, t = gy * w, xh = s * rstd:  dx = dres = round(rstd * (t - xh * mean(t * xh)) + gs),  dw = sum over rows of gy * xh
 //
+// Sums are fp32.  Where the sum of squares passes fp32 (values of 1e19 and more) it is formed again from the values times 2^-80.
+//
 // All of it is bound by memory: a row lives in the registers of the TPR threads that share it (NV 16-byte vectors each, the 16-bit types
 // packed), so every input is read once and every output written once.  Short rows are shared by 16 lanes or one wave (no barrier, several
-// rows per block), longer ones by a block of 256 to 1024.  Sums are fp32; dw is summed per block over the rows it owns (fp32 registers),
+// rows per block), longer ones by a block of 256 to 1024.  dw is summed per block over the rows it owns (fp32 registers),
 // then over the blocks in index order: reproducible.  Rows of more than 4096 vectors are walked by a block and read twice.
 // 8192 x 4096 bf16 with residual: forward 40 us (6.7 TB/s, part of it from the last-level cache), backward 53 us (5.1 TB/s, as a copy);
 // 6001 x 5000 to 8 bits 38 us (5.5 TB/s); 28800 x 64 fp32 5.7 and 9.2 us; one row of 4096 3.4 us, a launch.
@@ -52,6 +54,11 @@ template <int DT, bool TINY> __device__ __forceinline__ void ld_weight(const voi
         for (int e = 0; e < VE; ++e)
             if (c.at + e < d) f[e] = ((const float *)w)[c.at + e];
 }
+
+// rstd of a row whose sum of squares passes fp32, from the sum over its values times FAR; those squares are below 1e29, and a value whose own
+// is lost does not count beside the others.  (An inf: 0)
+constexpr float FAR = 0x1p-80f, FLT_TOP = 3.40282347e38f;
+__device__ __forceinline__ float far_rstd(float sum, int d, float eps) { return FAR / sqrtf(sum / (float)d + eps * FAR * FAR); }
 
 struct FwdArgs {
     long long rows; int d, wdtype; const char *x; long long ldx; const char *res; long long ldr; const void *w; float eps; char *s, *y;
@@ -101,7 +108,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
 #pragma unroll
         for (int e = 0; e < VE; ++e) acc += e >= c.skip ? f[e] * f[e] : 0.f;        // (what is past the row was read as 0)
     }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(acc, red) / (float)d + a.eps);
+    acc = row_sum<TPR>(acc, red);
+    float rstd = 1.f / sqrtf(acc / (float)d + a.eps);
+    if (__builtin_expect(acc > FLT_TOP, 0)) {                   // (the row's threads agree)
+        acc = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float f[VE];
+            unpack<DT>(v[j], f);
+            const Col<DT, TINY> c = col(j);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) { const float g = f[e] * FAR; acc += e >= c.skip ? g * g : 0.f; }
+        }
+        if constexpr (TPR > 64) __syncthreads();                // (all have read `red`)
+        rstd = far_rstd(row_sum<TPR>(acc, red), d, a.eps);
+    }
     if constexpr (!Q8) {
         if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
@@ -279,7 +300,13 @@ template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_ke
             if (a.s) st1<DT>(a.s, row * d + i, v);
             acc += v * v;
         }
-        const float rstd = 1.f / sqrtf(block_reduce<false>(acc, red) / (float)d + a.eps);
+        acc = block_reduce<false>(acc, red);
+        float rstd = 1.f / sqrtf(acc / (float)d + a.eps);
+        if (acc > FLT_TOP) {
+            acc = 0.f;
+            for (int i = threadIdx.x; i < d; i += LT) { const float v = at(i) * FAR; acc += v * v; }
+            rstd = far_rstd(block_reduce<false>(acc, red), d, a.eps);
+        }
         auto val = [&](int i) { return at(i) * rstd * weight1(a.w, a.wdtype, i); };
         if constexpr (!Q8) {
             if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;

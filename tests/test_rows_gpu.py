@@ -844,3 +844,47 @@ def test_the_norm_does_not_depend_on_the_call(count):
         assert torch.equal(train.clip_grad_norm_(gs, limit, out=out), n)
     assert torch.equal(train.clip_grad_norm_([g.clone() for g in gs], 1e9), n)
     assert abs(float(n) - 16777217.0) <= 1.0
+
+
+def far_rows(d, dtype, seed=0):
+    """an ordinary row; rows whose squares, or only their sum, pass fp32; a row near the type's largest values; one with an inf"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.rand(6, d, generator=g) * 2 - 1
+    x[:, 0] = 0.75
+    return (x * torch.tensor([1.0, 1.5e19, 1e30, 3.3e38, 1e25, 1.0])[:, None]).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("d", [1, 3, 7, 64, 120, 250, 520, 1000, 2050, 4100, 8200, 16000, 30000, 40001])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm_squares_past_fp32(dtype, d, residual):
+    base = far_rows(d, dtype, d)
+    x, r = ((base.double() * 0.6).to(dtype), (base.double() * 0.4).to(dtype)) if residual else (base, None)
+    x[5, d // 2] = math.inf
+    w, gy, gs = 1 + 0.1 * rnd(d, seed=3), rnd(6, d, dtype=dtype, seed=4), rnd(6, d, dtype=dtype, scale=0.1, seed=5) if residual else None
+    s, y64, dx64, mag, _, _ = norm64(x, r, w, 1e-6, gy, gs)
+    rstd = 1 / (s.double().square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    # rstd below the smallest normal number is off by half a step of 2^-149
+    rel = (chain(d) + 8) * U + torch.where(rstd > 0, 2.0 ** -150 / rstd, torch.zeros_like(rstd))
+    leaf, weight = x.to(DEV).requires_grad_(True), w.to(DEV)
+    out = modules.rms_norm(leaf, weight, residual=r.to(DEV) if residual else None)
+    y = out[0] if residual else out
+    u = half_step(dtype)
+    within(y, y64, u * y64.abs() + rel * y64.abs() + tiny(dtype), "y")
+    (dx,) = torch.autograd.grad(out, leaf, [gy.to(DEV), gs.to(DEV)] if residual else [gy.to(DEV)])
+    within(dx[:5], dx64[:5], u * dx64[:5].abs() + (2 * rel[:5] + (chain(d) + 16) * U) * mag[:5] + tiny(dtype), "dx")
+    weight = weight.requires_grad_(True)
+    z = modules.rms_norm(x[:5].to(DEV), weight, residual=r[:5].to(DEV) if residual else None)
+    (dw,) = torch.autograd.grad(z[0] if residual else z, weight, gy[:5].to(DEV))
+    *_, dw64, dwmag = norm64(x[:5], r[:5] if residual else None, w, 1e-6, gy[:5])
+    within(dw, dw64, U * dw64.abs() + (float(rel[:5].max()) + 16 * U) * dwmag, "dw")
+    for group in (0, 32, 512):
+        q, scale = modules.rms_norm_q8(x[:5].to(DEV), w.to(DEV), residual=r[:5].to(DEV) if residual else None, group=group)[:2]
+        g = group or d
+        ng = -(-d // g)
+        want = torch.nn.functional.pad(y64[:5].abs(), (0, ng * g - d)).view(5, ng, g).amax(-1) / 448
+        off = rel[:5] + 4 * U
+        within(scale, want, off * want, "scale")
+        cols = scale.cpu().double().repeat_interleave(g, 1)[:, :d]
+        err = (q.cpu().double() * cols - y64[:5]).abs()
+        assert float((err - (2.0 ** -4 * (1 + off) * y64[:5].abs()).clamp_min(2.0 ** -10 * 1.01 * cols) - 2 * off * y64[:5].abs()).max()) <= 0
