@@ -2,7 +2,7 @@
 //
 //   s = round(x + res)             the residual stream, kept in the inputs' type: the norm is of the stream as it is stored
 //   rstd = 1 / sqrt(mean(s^2) + eps),  y = round(s * rstd * w)
-//   8 bits: scale = max |s rstd w| / 448 over a group of columns (1 where that is below the smallest normal number), q = e4m3(s rstd w / scale)
+//   8 bits: scale = max |s rstd w| / 448 over a group of columns (1 where that quotient is 0), q = e4m3(s rstd w / scale)
 //   backward, t = gy * w, xh = s * rstd:  dx = dres = round(rstd * (t - xh * mean(t * xh)) + gs),  dw = sum over rows of gy * xh
 //
 // Sums are fp32.  Where the sum of squares passes fp32 (values of 1e19 and more) it is formed again from the values times 2^-80.
@@ -68,8 +68,18 @@ struct FwdArgs {
 __device__ __forceinline__ float scale_of(unsigned bits) {
     if (bits > 0x7f7fffffu) return __builtin_inff();
     const float sc = __uint_as_float(bits) / 448.f;
-    return sc < 1.17549435e-38f ? 1.f : sc;
+    return sc == 0.f ? 1.f : sc;
 }
+// v / sc = v * up * inv: the reciprocal of a scale below the smallest normal number may pass fp32, so both are taken 2^64 higher
+struct Divide {
+    float up, inv;
+    bool small;
+    __device__ __forceinline__ explicit Divide(float sc) : small(sc < 1.17549435e-38f) {
+        up = small ? 0x1p64f : 1.f;
+        inv = 1.f / (sc * up);
+    }
+    __device__ __forceinline__ float operator()(float v) const { return v * up * inv; }
+};
 
 template <int DT, int TPR, int NV, bool TINY, bool Q8>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4) void rms_fwd_kernel(FwdArgs a) {
@@ -162,14 +172,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
                     : lanes == 8 ? lanes_reduce<8>(b, MaxU{}) : lanes_reduce<4>(b, MaxU{});
             }
             if (!c.in) continue;
-            const float sc = scale_of(b), inv = 1.f / sc;
+            const float sc = scale_of(b);
+            const Divide by(sc);
             if (whole ? (t | j) == 0 : (t & (lanes - 1)) == 0) a.scale[row * ng + (whole ? 0 : (j * TPR + t) * VE / a.group)] = sc;
             float f[VE], w[VE];
             unpack<DT>(v[j], f);
             ld_weight<DT>(a.w, a.wdtype, c, d, w);
             unsigned u[VE / 4];
 #pragma unroll
-            for (int e = 0; e < VE; ++e) f[e] = f[e] * rstd * w[e] * inv;
+            for (int e = 0; e < VE; ++e) f[e] = f[e] * rstd * w[e];
+            if (by.small)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) f[e] *= by.up;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) f[e] *= by.inv;
 #pragma unroll
             for (int k = 0; k < VE / 4; ++k) u[k] = e4m3_pack4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
             if (!c.skip && c.at + VE <= d) __builtin_memcpy(q + c.at, u, VE);
@@ -318,18 +334,20 @@ template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_ke
                 unsigned m = 0u;
                 for (int i = g * a.group + lane; i < hi; i += 64) { const unsigned b = __float_as_uint(val(i)) & 0x7fffffffu; m = b > m ? b : m; }
                 m = row_reduce<64>(m, (unsigned *)nullptr, MaxU{});
-                const float sc = scale_of(m), inv = 1.f / sc;
+                const float sc = scale_of(m);
+                const Divide by(sc);
                 if (lane == 0) a.scale[row * ng + g] = sc;
-                for (int i = g * a.group + lane; i < hi; i += 64) a.q[row * d + i] = (unsigned char)e4m3_pack4(val(i) * inv, 0.f, 0.f, 0.f);
+                for (int i = g * a.group + lane; i < hi; i += 64) a.q[row * d + i] = (unsigned char)e4m3_pack4(by(val(i)), 0.f, 0.f, 0.f);
             }
         } else {
             unsigned m = 0u;
             for (int i = threadIdx.x; i < d; i += LT) { const unsigned b = __float_as_uint(val(i)) & 0x7fffffffu; m = b > m ? b : m; }
             __syncthreads();
             m = row_reduce<LT>(m, (unsigned *)red, MaxU{});
-            const float sc = scale_of(m), inv = 1.f / sc;
+            const float sc = scale_of(m);
+            const Divide by(sc);
             if (threadIdx.x == 0) a.scale[row] = sc;
-            for (int i = threadIdx.x; i < d; i += LT) a.q[row * d + i] = (unsigned char)e4m3_pack4(val(i) * inv, 0.f, 0.f, 0.f);
+            for (int i = threadIdx.x; i < d; i += LT) a.q[row * d + i] = (unsigned char)e4m3_pack4(by(val(i)), 0.f, 0.f, 0.f);
             __syncthreads();
         }
     }

@@ -697,7 +697,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6):
 def rms_norm_q8(x, weight=None, residual=None, eps=1e-6, group=0):
     """`rms_norm` whose output feeds an 8-bit product: -> (q float8_e4m3fn [..., d], scale float32 [..., ceil(d / group)]) and, with `residual`,
     the stream s as a third; q * scale is the norm's output.  One scale per row (group = 0) or per `group` columns (a power of two,
-    32 .. 512).  A group of zeros has scale 1, one with a NaN or inf scale inf.  For inference: refused where a gradient would be needed."""
+    32 .. 512).  A group of zeros (or whose largest value / 448 is 0 in float32) has scale 1, one with a NaN or inf scale inf.  For inference:
+    refused where a gradient would be needed."""
     q, scale, s = ops.rows().rms_norm_q8(x, weight, residual, eps, group)
     return (q, scale) if residual is None else (q, scale, s)
 

@@ -712,7 +712,7 @@ int i2p_kitti_image_build(int B, int out_h, int out_w, const void *table, float 
  * d <= I2P_MAX_ROW, rstd f32 [rows] = 1/sqrt(mean(s^2) + eps) (NULL: not wanted), y [rows,d] = round(s * rstd * w); w [d] of type wdtype (I2P_F32 or
  * dtype), NULL = ones.  s, y are dense.
  * _q8: q u8 [rows,d] = OCP e4m3 bits of s * rstd * w / scale, scale f32 [rows, ceil(d / group)] = max |s * rstd * w| / 448 over the group's
- * columns (1 where they are all zero); group a power of two, 32 .. 512, or 0 = the whole row.  A group with a NaN or inf has scale inf.
+ * columns (1 where that quotient is 0); group a power of two, 32 .. 512, or 0 = the whole row.  A group with a NaN or inf has scale inf.
  * _bwd: gy [rows,d], gs (gradient of s, NULL = none) -> dx [rows,d] (dense; the gradient of x and of res), dw [d] of type wdtype (NULL: not
  * wanted); s, rstd as the forward left them; scratch: i2p_rms_norm_bwd_scratch(rows, d) bytes, needed with dw.
  * --------------------------------------------------------------------------------------------- */

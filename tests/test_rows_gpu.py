@@ -888,3 +888,30 @@ def test_rms_norm_squares_past_fp32(dtype, d, residual):
         cols = scale.cpu().double().repeat_interleave(g, 1)[:, :d]
         err = (q.cpu().double() * cols - y64[:5]).abs()
         assert float((err - (2.0 ** -4 * (1 + off) * y64[:5].abs()).clamp_min(2.0 ** -10 * 1.01 * cols) - 2 * off * y64[:5].abs()).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("d,group", [(5, 32), (64, 0), (300, 64), (1000, 512), (4096, 128), (40001, 0), (40001, 128)])
+@pytest.mark.parametrize("weight", [1e-35, 1e-36, 1e-38, 1e-40, 1e-42, 1e-45])
+def test_rms_norm_q8_of_tiny_outputs(dtype, d, group, weight):
+    """scales below the smallest normal number are kept: 1 stands for a quotient that is 0, and for nothing else"""
+    x, w = rnd(3, d, dtype=dtype, seed=1), (torch.full((d,), weight, dtype=torch.float64) * (1 + 0.1 * rnd(d, seed=2).double())).float()
+    x[1] = 0
+    q, scale = modules.rms_norm_q8(x.to(DEV), w.to(DEV), group=group)
+    _, y = norm64(x, None, w, 1e-6)
+    g = group or d
+    ng = -(-d // g)
+    want = torch.nn.functional.pad(y.abs(), (0, ng * g - d)).view(3, ng, g).amax(-1) / 448
+    rel, step = (chain(d) + 12) * U, 2.0 ** -149
+    scale = scale.cpu().double()
+    # the largest value is off by half a step of 2^-149 at most, the quotient by another half
+    zero = scale == 1
+    assert (want[zero] <= 0.51 * step).all() and zero[1].all() and (want[~zero] >= 0.49 * step).all()
+    within(scale[~zero], want[~zero], rel * want[~zero] + 0.51 * step, "scale")
+    cols = scale.repeat_interleave(g, 1)[:, :d]
+    dead = zero.repeat_interleave(g, 1)[:, :d]
+    assert not q.cpu().double()[dead].any()
+    # a scale rounded down by half a step saturates its largest values: 448 half steps; the value itself is off by half a step
+    err = (q.cpu().double() * cols - y).abs()
+    bound = (2.0 ** -4 * (1 + rel) * y.abs()).clamp_min(2.0 ** -10 * 1.01 * cols) + 2 * rel * y.abs() + (448 * 0.51 + 1) * step
+    assert float((err - bound).masked_fill(dead, -1.0).max()) <= 0
