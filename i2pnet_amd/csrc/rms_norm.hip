@@ -5,7 +5,8 @@
 //   8 bits: scale = max |s rstd w| / 448 over a group of columns (1 where that quotient is 0), q = e4m3(s rstd w / scale)
 //   backward, t = gy * w, xh = s * rstd:  dx = dres = round(rstd * (t - xh * mean(t * xh)) + gs),  dw = sum over rows of gy * xh
 //
-// Sums are fp32.  Where the sum of squares passes fp32 (values of 1e19 and more) it is formed again from the values times 2^-80.
+// Sums are fp32.  Where the sum of squares passes fp32 (values of 1e19 and more), or would lose digits below it and eps does not cover that
+// (values of 1e-12 and less with an eps as small), it is formed again from scaled values.
 //
 // All of it is bound by memory: a row lives in the registers of the TPR threads that share it (NV 16-byte vectors each, the 16-bit types
 // packed), so every input is read once and every output written once.  Short rows are shared by 16 lanes or one wave (no barrier, several
@@ -55,10 +56,15 @@ template <int DT, bool TINY> __device__ __forceinline__ void ld_weight(const voi
             if (c.at + e < d) f[e] = ((const float *)w)[c.at + e];
 }
 
-// rstd of a row whose sum of squares passes fp32, from the sum over its values times FAR; those squares are below 1e29, and a value whose own
-// is lost does not count beside the others.  (An inf: 0)
-constexpr float FAR = 0x1p-80f, FLT_TOP = 3.40282347e38f;
-__device__ __forceinline__ float far_rstd(float sum, int d, float eps) { return FAR / sqrtf(sum / (float)d + eps * FAR * FAR); }
+// Rows of d <= 2^26 whose squares fp32 does not hold are summed again from their values times `by`:
+//   2^-80 where the sum is inf: squares below 1e29, and a value whose own is lost does not count beside the others.  (A value inf: rstd 0)
+//   2^90 where mean + eps is at most 2^-80: a sum below 2^126, and squares of the smallest subnormal numbers are 2^-118
+struct Far {
+    float by;
+    bool is;
+    __device__ __forceinline__ Far(float sum, float var) : by(sum > 3.40282347e38f ? 0x1p-80f : 0x1p90f), is(sum > 3.40282347e38f || var <= 0x1p-80f) {}
+    __device__ __forceinline__ float rstd(float sum, int d, float eps) const { return by / sqrtf(sum / (float)d + eps * by * by); }
+};
 
 struct FwdArgs {
     long long rows; int d, wdtype; const char *x; long long ldx; const char *res; long long ldr; const void *w; float eps; char *s, *y;
@@ -119,8 +125,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
         for (int e = 0; e < VE; ++e) acc += e >= c.skip ? f[e] * f[e] : 0.f;        // (what is past the row was read as 0)
     }
     acc = row_sum<TPR>(acc, red);
-    float rstd = 1.f / sqrtf(acc / (float)d + a.eps);
-    if (__builtin_expect(acc > FLT_TOP, 0)) {                   // (the row's threads agree)
+    const float var = acc / (float)d + a.eps;
+    float rstd = 1.f / sqrtf(var);
+    const Far far(acc, var);
+    if (__builtin_expect(far.is, 0)) {                          // (the row's threads agree)
         acc = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -128,10 +136,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, NV < 3 ? 8 : NV < 4 ? 6 : 4)
             unpack<DT>(v[j], f);
             const Col<DT, TINY> c = col(j);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) { const float g = f[e] * FAR; acc += e >= c.skip ? g * g : 0.f; }
+            for (int e = 0; e < VE; ++e) { const float g = f[e] * far.by; acc += e >= c.skip ? g * g : 0.f; }
         }
         if constexpr (TPR > 64) __syncthreads();                // (all have read `red`)
-        rstd = far_rstd(row_sum<TPR>(acc, red), d, a.eps);
+        rstd = far.rstd(row_sum<TPR>(acc, red), d, a.eps);
     }
     if constexpr (!Q8) {
         if (a.rstd && t == 0) a.rstd[row] = rstd;
@@ -317,11 +325,13 @@ template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_ke
             acc += v * v;
         }
         acc = block_reduce<false>(acc, red);
-        float rstd = 1.f / sqrtf(acc / (float)d + a.eps);
-        if (acc > FLT_TOP) {
+        const float var = acc / (float)d + a.eps;
+        float rstd = 1.f / sqrtf(var);
+        const Far far(acc, var);
+        if (far.is) {
             acc = 0.f;
-            for (int i = threadIdx.x; i < d; i += LT) { const float v = at(i) * FAR; acc += v * v; }
-            rstd = far_rstd(block_reduce<false>(acc, red), d, a.eps);
+            for (int i = threadIdx.x; i < d; i += LT) { const float v = at(i) * far.by; acc += v * v; }
+            rstd = far.rstd(block_reduce<false>(acc, red), d, a.eps);
         }
         auto val = [&](int i) { return at(i) * rstd * weight1(a.w, a.wdtype, i); };
         if constexpr (!Q8) {

@@ -915,3 +915,33 @@ def test_rms_norm_q8_of_tiny_outputs(dtype, d, group, weight):
     err = (q.cpu().double() * cols - y).abs()
     bound = (2.0 ** -4 * (1 + rel) * y.abs()).clamp_min(2.0 ** -10 * 1.01 * cols) + 2 * rel * y.abs() + (448 * 0.51 + 1) * step
     assert float((err - bound).masked_fill(dead, -1.0).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("d", [1, 7, 64, 250, 520, 4100, 16000, 30000, 40001])
+@pytest.mark.parametrize("eps", [0.0, 1e-37])
+def test_rms_norm_squares_below_fp32(dtype, d, eps):
+    """rows whose squares are too small for fp32, next to ordinary ones, where eps does not cover them"""
+    x = (far_rows(d, torch.float64, d) / far_rows(d, torch.float64, d).abs().amax(-1, keepdim=True) *
+         torch.tensor([1.0, 1e-12, 1e-18, 1e-22, 1e-30, 1e-37], dtype=torch.float64)[:, None]).to(dtype)
+    w, gy = 1 + 0.1 * rnd(d, seed=3), rnd(6, d, dtype=dtype, seed=4)
+    s, y64, dx64, mag, dw64, dwmag = norm64(x, None, w, eps, gy)
+    rel = (chain(d) + 10) * U
+    leaf, weight = x.to(DEV).requires_grad_(True), w.to(DEV).requires_grad_(True)
+    y = modules.rms_norm(leaf, weight, eps=eps)
+    within(y, y64, half_step(dtype) * y64.abs() + rel * y64.abs() + tiny(dtype), "y")
+    dx, dw = torch.autograd.grad(y, [leaf, weight], gy.to(DEV))
+    # rows of 1e-37 have gradients up to 1e37 times a few: within the types' range
+    within(dx, dx64, half_step(dtype) * dx64.abs() + (2 * rel + (chain(d) + 16) * U) * mag + tiny(dtype), "dx")
+    within(dw, dw64, U * dw64.abs() + (rel + 16 * U) * dwmag, "dw")
+    q, scale = modules.rms_norm_q8(x.to(DEV), w.to(DEV), eps=eps)
+    want = y64.abs().amax(-1, keepdim=True) / 448
+    within(scale, want, (rel + 4 * U) * want, "scale")
+    err = (q.cpu().double() * scale.cpu().double() - y64).abs()
+    assert float((err - (2.0 ** -4 * (1 + rel) * y64.abs()).clamp_min(2.0 ** -10 * 1.01 * scale.cpu().double()) - 2 * rel * y64.abs()).max()) <= 0
+
+
+def test_rms_norm_of_zeros_without_eps():
+    y = modules.rms_norm(torch.zeros(2, 40, device=DEV), None, eps=0.0)
+    assert torch.isnan(y).all()                             # 0 / 0, as the formula has it
+    assert not modules.rms_norm(torch.zeros(2, 40, device=DEV), None, eps=1e-38).any()
