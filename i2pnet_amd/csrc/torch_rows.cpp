@@ -337,8 +337,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits, 
 }
 
 // ---- gradient norm ---------------------------------------------------------------------------------------------------------------
-// the gradients meant by one tensor or an iterable of them: a parameter's .grad (where it has one), or the gradient tensor itself
-std::vector<Tensor> grad_list(const py::object &parameters) {
+// the gradients meant by one tensor or an iterable of them: a parameter's .grad (where it has one), or the gradient tensor itself; `device`:
+// of the first of them
+std::vector<Tensor> grad_list(const py::object &parameters, std::optional<c10::Device> *device = nullptr) {
     std::vector<Tensor> grads;
     auto add = [&](PyObject *o) {
         if (Py_TYPE(o) == (PyTypeObject *)THPVariableClass) {
@@ -351,6 +352,7 @@ std::vector<Tensor> grad_list(const py::object &parameters) {
                     "parameters (leaves) or gradient tensors are wanted (got ", Py_TYPE(o)->tp_name, " without a gradient)");
         TORCH_CHECK(t.is_leaf(), "parameters (leaves) or gradient tensors are wanted (got a tensor that an operation made and that requires a gradient)");
         if (t.grad().defined()) grads.push_back(t.grad());
+        else if (device && !*device) *device = t.device();
     };
     if (THPVariable_Check(parameters.ptr())) { add(parameters.ptr()); return grads; }
     const auto list = py::reinterpret_steal<py::object>(PySequence_Fast(parameters.ptr(), "parameters, gradient tensors or one of them are wanted"));
@@ -403,10 +405,14 @@ Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optio
     return norm;
 }
 
-// the same on parameters or gradients; nothing where there is no gradient
-OptTensor clip_parameters(const py::object &parameters, int64_t kind, std::optional<double> max_norm, const OptTensor &out) {
-    const std::vector<Tensor> grads = grad_list(parameters);
-    if (grads.empty()) return std::nullopt;
+// the same on parameters or gradients.  Parameters without gradients have a norm of 0 on their device; no parameter at all: on the current one
+Tensor clip_parameters(const py::object &parameters, int64_t kind, std::optional<double> max_norm, const OptTensor &out) {
+    std::optional<c10::Device> device;
+    const std::vector<Tensor> grads = grad_list(parameters, &device);
+    if (grads.empty()) {
+        TORCH_CHECK(!max_norm || !out || out->numel() == 0, "out must be empty: there is no gradient");
+        return at::zeros({}, at::TensorOptions().dtype(at::kFloat).device(device.value_or(c10::Device(c10::kCUDA))));
+    }
     return clip_grad_norm(grads, kind, max_norm, out);
 }
 
@@ -424,7 +430,7 @@ PYBIND11_MODULE(_torch_rows, m) {
     m.def("token_logprobs", wrap_pybind_function_no_gil(token_logprobs));
     m.def("token_logprobs_forward", wrap_pybind_function_no_gil(token_logprobs_forward));
     m.def("token_logprobs_backward", wrap_pybind_function_no_gil(token_logprobs_backward));
-    m.def("grad_list", wrap_pybind_function(grad_list));
+    m.def("grad_list", wrap_pybind_function([](const py::object &parameters) { return grad_list(parameters); }));
     m.def("clip_grad_norm", wrap_pybind_function(clip_grad_norm));
     m.def("clip_parameters", wrap_pybind_function(clip_parameters));
 }

@@ -154,10 +154,9 @@ def _norm_kind(norm_type):
 
 
 def grad_norm(parameters, norm_type=2.0):
-    """Global norm (2, or inf: the largest magnitude) of the gradients of `parameters` -> float32 0-d tensor on their device; the host does
-    not wait.  `parameters`: parameters, whose .grad is meant (those without one are skipped), or gradient tensors themselves."""
-    total = ops.rows().clip_parameters(parameters, _norm_kind(norm_type), None, None)
-    return torch.zeros((), device="cuda") if total is None else total
+    """Global norm (2, or inf: the largest magnitude) of the gradients of `parameters` -> float32 0-d tensor on their device (0 where
+    there is no gradient); the host does not wait.  `parameters`: parameters, whose .grad is meant (those without one are skipped), or gradient tensors themselves."""
+    return ops.rows().clip_parameters(parameters, _norm_kind(norm_type), None, None)
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, out=None):
@@ -173,17 +172,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative (got {max_norm})")
     if error_if_nonfinite:
+        parameters = parameters if isinstance(parameters, torch.Tensor) else list(parameters)
         grads = _grad_list(parameters)
         if grads and not bool(torch.isfinite(ops.rows().clip_grad_norm(grads, kind, None, None))):
             raise RuntimeError("the global norm of the gradients is not finite: they were not clipped")
-        total = ops.rows().clip_grad_norm(grads, kind, max_norm, out) if grads else None
-    else:
-        total = ops.rows().clip_parameters(parameters, kind, max_norm, out)
-    if total is None:
-        if out is not None and out.numel():
-            raise RuntimeError("out must be empty: there is no gradient")
-        return torch.zeros((), device="cuda")
-    return total
+    return ops.rows().clip_parameters(parameters, kind, max_norm, out)
 
 
 # what a step reads of a loader sample dict (kitti_odometry_corr_lidarnone_proj.py:757-789 also carries strings

@@ -205,3 +205,14 @@ def test_a_backward_pass_that_is_being_traced_is_refused():
             torch.jit.trace(f, (s,), check_trace=False)
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(f)(s)
+
+
+def test_parameters_without_gradients_have_a_norm_of_zero_on_their_device():
+    p = [torch.nn.Parameter(torch.ones(3)), torch.nn.Parameter(torch.ones(2), requires_grad=False)]
+    for f in (lambda a: train.grad_norm(a), lambda a: train.clip_grad_norm_(a, 1.0), lambda a: train.clip_grad_norm_(a, 1.0, error_if_nonfinite=True),
+              lambda a: train.clip_grad_norm_(a, 1.0, out=torch.zeros(0))):
+        for a in (p, p[0], iter(p), p[1:]):
+            n = f(a)
+            assert n.device.type == "cpu" and n.dtype == torch.float32 and n.shape == () and float(n) == 0.0
+    with pytest.raises(RuntimeError, match="out must be empty"):
+        train.clip_grad_norm_(p, 1.0, out=torch.zeros(1))
