@@ -1,6 +1,7 @@
 """Row operators without a GPU: what is refused before any launch."""
 import ctypes as C
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -216,3 +217,30 @@ def test_parameters_without_gradients_have_a_norm_of_zero_on_their_device():
             assert n.device.type == "cpu" and n.dtype == torch.float32 and n.shape == () and float(n) == 0.0
     with pytest.raises(RuntimeError, match="out must be empty"):
         train.clip_grad_norm_(p, 1.0, out=torch.zeros(1))
+
+
+def test_the_longest_row():
+    """I2P_MAX_ROW itself: the row after it is refused, and by the tensor checks too"""
+    for d, ok in ((1 << 26, True), ((1 << 26) + 1, False)):
+        for name, args in (("i2p_rms_norm_fwd", (0, d, 1, 0, None, d, None, 0, None, 1e-6, None, None, None)),
+                           ("i2p_rms_norm_q8", (0, d, 1, 0, None, d, None, 0, None, 1e-6, 0, None, None, None))):
+            if ok:
+                call(name, *args)                           # (no rows is no work)
+            else:
+                with pytest.raises(_lib.I2POpsError, match=BAD):
+                    call(name, *args)
+    with pytest.raises(_lib.I2POpsError, match=BAD):
+        call("i2p_rms_norm_bwd", 1, (1 << 26) + 1, 1, 0, P, (1 << 26) + 1, P, (1 << 26) + 1, None, 0, None, P, P, None, None)
+    assert _lib.helper("i2p_rms_norm_bwd_scratch", 1, 1 << 26) == 4 << 26
+
+
+def test_limits_are_the_header_s():
+    text = (Path(__file__).resolve().parent.parent / "include" / "i2p_ops.h").read_text()
+    assert f"#define I2P_MAX_TOP {ops.MAX_TOP}\n" in text and "#define I2P_MAX_CANDIDATES (1 << 21)\n" in text and "#define I2P_MAX_ROW (1 << 26)\n" in text
+    a = dict(rows=0, v=100, dtype=1, x=None, ldx=1 << 22, ids=None, ignore=-100, top=ops.MAX_TOP, logp=None, entropy=None, stat=None, top_logp=None, top_ids=None,
+             scratch=None)
+    call("i2p_token_logprobs_fwd", *a.values())
+    call("i2p_token_logprobs_fwd", *(a | dict(v=1 << 21)).values())
+    for change in (dict(top=ops.MAX_TOP + 1), dict(v=(1 << 21) + 1)):
+        with pytest.raises(_lib.I2POpsError, match=BAD):
+            call("i2p_token_logprobs_fwd", *(a | change).values())
