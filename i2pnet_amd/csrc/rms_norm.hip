@@ -324,14 +324,14 @@ template <int DT, bool Q8> __global__ __launch_bounds__(LT) void rms_fwd_long_ke
             if (a.s) st1<DT>(a.s, row * d + i, v);
             acc += v * v;
         }
-        acc = block_reduce<false>(acc, red);
+        acc = block_total(acc, red);
         const float var = acc / (float)d + a.eps;
         float rstd = 1.f / sqrtf(var);
         const Far far(acc, var);
         if (far.is) {
             acc = 0.f;
             for (int i = threadIdx.x; i < d; i += LT) { const float v = at(i) * far.by; acc += v * v; }
-            rstd = far.rstd(block_reduce<false>(acc, red), d, a.eps);
+            rstd = far.rstd(block_total(acc, red), d, a.eps);
         }
         auto val = [&](int i) { return at(i) * rstd * weight1(a.w, a.wdtype, i); };
         if constexpr (!Q8) {
@@ -379,7 +379,7 @@ template <int DT> __global__ __launch_bounds__(LT) void rms_bwd_long_kernel(BwdA
             acc += c * weight1(a.w, a.wdtype, i);
             if (my) my[i] += c;
         }
-        const float mean = block_reduce<false>(acc, red) / (float)d;
+        const float mean = block_total(acc, red) / (float)d;
         for (int i = threadIdx.x; i < d; i += LT) {
             float v = rstd * (ld1<DT>(gy, i) * weight1(a.w, a.wdtype, i) - ld1<DT>(s, i) * rstd * mean);
             if (a.gs) v += ld1<DT>(gs, i);

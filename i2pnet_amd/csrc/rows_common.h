@@ -113,14 +113,14 @@ struct MaxU { __device__ __forceinline__ unsigned operator()(unsigned a, unsigne
 template <int N> __device__ __forceinline__ float lanes_sum(float v) { return __uint_as_float(lanes_reduce<N>(__float_as_uint(v), AddF{})); }
 template <int N> __device__ __forceinline__ float lanes_max(float v) { return __uint_as_float(lanes_reduce<N>(__float_as_uint(v), MaxF{})); }
 
-// sum / maximum over the block's waves; every thread gets the result.  red: one float per wave.  (All threads of the block call it; the
-// trailing barrier lets the caller use `red` again.)
-template <bool MAX> __device__ __forceinline__ float block_reduce(float v, float *red) {
-    v = MAX ? lanes_max<64>(v) : lanes_sum<64>(v);
+// sum over the block's waves; every thread gets the result.  red: one float per wave.  (All threads of the block call it; the trailing barrier
+// lets the caller use `red` again.)
+__device__ __forceinline__ float block_total(float v, float *red) {
+    v = lanes_sum<64>(v);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float t = red[0];
-    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) t = MAX ? fmaxf(t, red[w]) : t + red[w];
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) t += red[w];
     __syncthreads();
     return t;
 }

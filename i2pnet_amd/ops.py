@@ -21,7 +21,6 @@ _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
 _BF16 = torch.bfloat16
 BN_REPLICAS = 32          # I2P_BN_REPLICAS in include/i2p_ops.h
 MAX_TOP = 32              # I2P_MAX_TOP
-MAX_CANDIDATES = 1 << 21  # I2P_MAX_CANDIDATES
 
 # ---- activation storage precision of the fused layer chains ---------------------------------------------------------
 # "fp32" (default; BASELINE configs[1], the reference's precision) or "bf16": the pre-BN
