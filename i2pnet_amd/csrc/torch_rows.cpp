@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -373,11 +374,12 @@ Tensor clip_grad_norm(const std::vector<Tensor> &grads, int64_t kind, std::optio
     std::vector<const void *> ptrs(n);
     std::vector<long long> sizes(n);
     std::vector<int> types(n);
+    const bool forward_mode = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;       // (asking 254 tensors takes 1 .. 3 us)
     std::vector<Tensor> copies;                 // (in place a flagged sign changes nothing: what is scaled is its negative)
     long long total = 0;
     for (int i = 0; i < n; ++i) {
         const Tensor &g = grads[i];
-        primal(g, "a gradient");
+        if (forward_mode) primal(g, "a gradient");
         types[i] = type_of(g);
         TORCH_CHECK(types[i] >= 0, "gradients must be float32, bfloat16 or float16 (got ", g.scalar_type(), ")");
         TORCH_CHECK(g.is_cuda() && g.device() == device, "gradients must be cuda tensors on one device (got ", g.device(), ")");
