@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -123,17 +124,19 @@ struct Rows {
     }
 };
 
-// gradients of a backward pass that cannot be differentiated again: says so where that is tried
-variable_list once(variable_list g) {
+// Gradients of a backward pass that cannot be differentiated again.  They get a history that says so when it is walked: an error node above all
+// that they depend on, the operator's inputs and the gradients `from` that came in, so that no way to a second derivative takes it for zero
+variable_list once(variable_list g, const variable_list &from) {
     if (!at::GradMode::is_enabled()) return g;
-    variable_list in;
+    torch::autograd::edge_list above = torch::autograd::collect_next_edges(from);
+    const auto inputs = torch::autograd::get_current_node()->next_edges();
+    above.insert(above.end(), inputs.begin(), inputs.end());
+    const auto error = std::make_shared<torch::autograd::Error>("trying to differentiate twice a function marked once_differentiable", std::move(above));
     for (auto &t : g)
-        if (t.defined()) in.push_back(t.detach().requires_grad_(true));
-    const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function marked once_differentiable", in.size());
-    variable_list out = error->apply(std::move(in));
-    size_t k = 0;
-    for (auto &t : g)
-        if (t.defined()) t = out[k++];
+        if (t.defined()) {
+            t = t.detach();
+            torch::autograd::set_history(t, error);
+        }
     return g;
 }
 
@@ -233,9 +236,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         OptTensor weight, gs;
         if (saved.size() > 2) weight = saved[2];
         if (residual && g[1].defined()) gs = g[1];
-        if (!g[0].defined()) return once({gs.value_or(Tensor()), residual ? gs.value_or(Tensor()) : Tensor(), Tensor(), Tensor()});
+        if (!g[0].defined()) return once({gs.value_or(Tensor()), residual ? gs.value_or(Tensor()) : Tensor(), Tensor(), Tensor()}, g);
         auto [dx, dw] = rms_norm_backward(saved[0], weight, saved[1], g[0], gs, weight && ctx->needs_input_grad(residual ? 2 : 1));
-        return once({dx, residual ? dx : Tensor(), dw.value_or(Tensor()), Tensor()});
+        return once({dx, residual ? dx : Tensor(), dw.value_or(Tensor()), Tensor()}, g);
     }
 };
 
@@ -324,7 +327,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
         const variable_list s = ctx->get_saved_variables();
         const Tensor dx = token_logprobs_backward(s[0], s[1], ctx->saved_data["ignore"].toInt(), s[2], s[3], g[0].defined() ? OptTensor(g[0]) : OptTensor(),
                                                   g[1].defined() ? OptTensor(g[1]) : OptTensor());
-        return once({dx.view(ctx->saved_data["shape"].toIntVector()), Tensor(), Tensor(), Tensor()});
+        return once({dx.view(ctx->saved_data["shape"].toIntVector()), Tensor(), Tensor(), Tensor()}, g);
     }
 };
 

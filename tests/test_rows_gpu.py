@@ -945,3 +945,42 @@ def test_rms_norm_of_zeros_without_eps():
     y = modules.rms_norm(torch.zeros(2, 40, device=DEV), None, eps=0.0)
     assert torch.isnan(y).all()                             # 0 / 0, as the formula has it
     assert not modules.rms_norm(torch.zeros(2, 40, device=DEV), None, eps=1e-38).any()
+
+
+def twice_cases():
+    w, ids, r = rnd(9, seed=2).to(DEV), torch.zeros(3, dtype=torch.long, device=DEV), rnd(3, 9, seed=3).to(DEV)
+    return {"norm": lambda a: modules.rms_norm(a, w), "norm, rows apart": lambda a: modules.rms_norm(a.t().contiguous().t(), w),
+            "norm, residual": lambda a: modules.rms_norm(a, w, residual=r)[0], "stream": lambda a: modules.rms_norm(r, w, residual=a)[1],
+            "norm of the stream": lambda a: modules.rms_norm(modules.rms_norm(r, w, residual=a)[1], None),
+            "logp": lambda a: loss.token_logprobs(a, ids).logp, "entropy": lambda a: loss.token_logprobs(a, ids).entropy}
+
+
+@pytest.mark.parametrize("name", ["norm", "norm, rows apart", "norm, residual", "stream", "norm of the stream", "logp", "entropy"])
+def test_second_derivatives_are_refused_by_every_way(name):
+    """and are not taken for zero: with respect to the input, the weight and the gradient that came in, by autograd.grad and torch.autograd.functional"""
+    f, a = twice_cases()[name], rnd(3, 9, seed=1).to(DEV).requires_grad_(True)
+    refused = lambda: pytest.raises(RuntimeError, match="once_differentiable")
+    y = f(a)
+    gy = torch.ones_like(y).requires_grad_(True)
+    (g,) = torch.autograd.grad(y, a, gy, create_graph=True)
+    for what in (a, gy):
+        for unused in (False, True):
+            with refused():
+                torch.autograd.grad(g.square().sum(), what, retain_graph=True, allow_unused=unused)
+    with refused():
+        torch.autograd.functional.hessian(lambda b: f(b).sum(), a.detach())
+    with refused():
+        torch.autograd.functional.vhp(lambda b: f(b).square().sum(), a.detach(), torch.ones_like(a))
+    with refused():
+        torch.autograd.functional.jvp(f, a.detach(), torch.ones_like(a))
+    # the first derivatives that carry that refusal are the ordinary ones
+    (plain,) = torch.autograd.grad(f(a), a, gy.detach())
+    assert torch.equal(g, plain) and not plain.requires_grad
+    assert torch.autograd.functional.jacobian(lambda b: f(b).sum(0), a.detach()).shape[-2:] == a.shape
+
+
+def test_second_derivatives_of_the_weight_are_refused():
+    x, w = rnd(3, 9, seed=1).to(DEV), rnd(9, seed=2).to(DEV).requires_grad_(True)
+    (g,) = torch.autograd.grad(modules.rms_norm(x, w).square().sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.sum(), w, allow_unused=True)
