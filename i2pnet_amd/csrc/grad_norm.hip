@@ -7,9 +7,9 @@
 // depends on the list's sizes and types alone: the norm is the same with clipping and without, in place or not.  A NaN or inf reaches the total and,
 // through c, every gradient.
 //
-// Bound by memory where there is much (300 M elements, bf16 and fp32, into the flat buffer: norm 165 us = 4.3 TB/s read, clipping 371 us =
-// 5.2 TB/s read and written) and by two launches where there is little (254 tensors of 845 k elements in place: 6.0 + 3.3 us; the host takes
-// 22 us to list them).
+// Bound by memory where there is much (300 M elements, bf16 and fp32, into the flat buffer: norm 164 us = 4.3 TB/s read, clipping 370 us =
+// 5.2 TB/s read and written) and by two launches where there is little (254 tensors of 845 k elements in place: 4.9 + 2.8 us of a call of 20:
+// the rest is the host, which lists them).
 #include "rows_common.h"
 #include <algorithm>
 #include <new>
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(T) void grad_clip_kernel(Table<OUT> t, float max_no
 inline long long chunks_of(long long numel, int chunk) { return (numel + chunk - 1) / chunk; }
 
 // A chunk is what a block reads (at most 65536 elements: 16 bits of `ptr` tell the last one's length): 4096 elements, one batch of loads a
-// thread, while there are few; else 16384 (300 M elements: 531 us in all, 577 with 65536)
+// thread, while there are few; else 16384 (300 M elements: 541 us in all, 583 with 65536)
 inline int chunk_for(int n, const long long *numel) {
     long long total = 0;
     for (int i = 0; i < n; ++i) total += numel[i];

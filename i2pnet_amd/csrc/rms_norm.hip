@@ -11,9 +11,12 @@
 // All of it is bound by memory: a row lives in the registers of the TPR threads that share it (NV 16-byte vectors each, the 16-bit types
 // packed), so every input is read once and every output written once.  Short rows are shared by 16 lanes or one wave (no barrier, several
 // rows per block), longer ones by a block of 256 to 1024.  dw is summed per block over the rows it owns (fp32 registers),
-// then over the blocks in index order: reproducible.  Rows of more than 4096 vectors are walked by a block and read twice.
-// 8192 x 4096 bf16 with residual: forward 40 us (6.7 TB/s, part of it from the last-level cache), backward 53 us (5.1 TB/s, as a copy);
-// 6001 x 5000 to 8 bits 38 us (5.5 TB/s); 28800 x 64 fp32 5.7 and 9.2 us; one row of 4096 3.4 us, a launch.
+// then over the blocks in index order: reproducible.
+// 8192 x 4096 bf16 with residual: forward 45 us (6.0 TB/s, part of it from the last-level cache), backward 58 us (4.6 TB/s) and 4.6 for dw;
+// 6001 x 5000 to 8 bits 48 us (4.4 TB/s); 28800 x 64 fp32 7.7, 7.1 and 3.6 us; one row of 4096 2.6 us.
+// Not of that form: rows of more than 4096 vectors, and fp32 rows of more than 256 columns in groups of 512 (two waves' vectors), are walked
+// by a block, one element a thread, and read twice (three times to 8 bits).  The backward of 16-bit rows of more than 16384 columns keeps its
+// four vectors a thread, with their weight gradients, partly in scratch memory (80 registers).
 #include "rows_common.h"
 #include <algorithm>
 
@@ -393,8 +396,8 @@ inline bool types_ok(int dtype, int wdtype) {
 }
 
 // Blocks of the backward pass for `rows` rows (or runs of rows) of a block of `threads`: as many as run at once (four waves a SIMD), but no
-// more than 2^21 partial weight gradients, whose write and read cost as much as a row's (8192 x 4096 bf16: 512 blocks 59 us, 1024 61, 2048 75;
-// 30000 x 1000: 512 blocks 46 us, 1024 44, 2048 48)
+// more than 2^21 partial weight gradients, whose write and read cost as much as a row's (8192 x 4096 bf16: 512 blocks 63 us in both
+// launches, 1024 67, 2048 70; 30000 x 1000: 512 blocks 65 us, 1024 51, 2048 55)
 inline long long bwd_blocks(long long rows, int d, int threads) {
     const long long most = std::min(262144ll / threads, std::max(256ll, (1ll << 21) / d));
     return std::min(rows, most);
@@ -414,8 +417,8 @@ template <int DT, bool BWD, class F> bool by_width(int d, F f) {
     if (n <= 128) I2P_ROW(64, 2, false)
     if (n <= 256) I2P_ROW(256, 1, false)
     if constexpr (BWD) {
-        // the weight gradients double the registers of a vector: more threads with one vector each (8192 x 4096 bf16 as 256 x 2: 55.9 us,
-        // 512 x 1: 52.6; 4000 x 8000 as 512 x 2: 76.6, 1024 x 1: 50.6), unless many of them would have none (15000 x 2100: 55.6, 62.1)
+        // the weight gradients double the registers of a vector: more threads with one vector each (8192 x 4096 bf16 as 256 x 2: 62 us,
+        // 512 x 1: 58; 4000 x 8000 as 512 x 2: 85, 1024 x 1: 57), unless many of them would have none (15000 x 2100: 65, 74)
         if (n <= 384) I2P_ROW(256, 2, false)
         if (n <= 512) I2P_ROW(512, 1, false)
         if (n <= 1024) I2P_ROW(1024, 1, false)

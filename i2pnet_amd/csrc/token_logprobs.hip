@@ -6,16 +6,17 @@
 // The maximum and L are kept apart for the backward pass: rounded into one number, scores of a few hundred would lose the digits of L.
 // A row without candidates (all -inf): logp -inf, H 0, gradient 0.  +inf or NaN in a row: logp, H, top_logp and the gradient are NaN.
 //
-// Forward: reads the scores once.  A row of more than 128 scores, or a slice of a long one, stays in the registers of a wave, of 4 or of 16 waves (at most 32 scores a
-// thread, 64 of the 16-bit types), so that the maximum is known before the first exponential; slices leave (max, S, sum z e^z) and their k
-// best in the workspace and a second launch joins them.  8192 x 131072 bf16: 455 us, 4.7 TB/s (a plain sum of that much reads 4.0 TB/s here);
-// the vector units are 80 % busy beside it, some 8 instructions a score (PMC on slices of 8192: 413 a wave of 32 scores a lane).  4096 x 32000:
-// 72 us, of which about 15 are the first and the last round of blocks.
+// Forward: reads the scores once.  A row of more than 128 scores, or a slice of a long one, stays in the registers of a wave, of 4 or of 16
+// waves (at most 32 scores a thread, 64 of the 16-bit types), so that the maximum is known before the first exponential; slices leave (max, S,
+// sum z e^z) and their k best in the workspace and a second launch joins them.  8192 x 131072 bf16: 430 .. 470 us, 4.6 .. 5.0 TB/s (a plain sum
+// of that much reads 4.0 TB/s here), and 13 to join; a wave issues 715 vector instructions for 64 scores a lane, in 75 % of the cycles, and the
+// exponentials among them take four times a slot.  4096 x 32000: 58 + 6 us; a wave's fixed part weighs more in shorter slices (387 for 28 scores a lane).
 // Best alternatives: the threads' maxima give 64 group maxima; the k-th largest of those (to 16 bits) is a value that at least k scores reach
 // and that few others do.  The scores that reach it go to LDS and are ranked by counting.  Rows with many equal scores (or a NaN) overflow
-// that list and are searched k times instead.  10000 x 2000 fp32: 15.4 us without alternatives, 19.6 with 8, 24.8 with 32.
-// Backward: elementwise from the saved maximum, L and H; bound by reading the scores again and writing as much: 8192 x 131072 bf16 725 us,
-// 5.9 TB/s.
+// that list and are searched k times instead.  10000 x 2000 fp32: 15.2 us without alternatives, 20.0 with 8, 25.0 with 32; 777 x 50001 fp16:
+// 22 + 4 us without, 26 + 5 with 5 (387 and 497 vector instructions a wave).
+// Backward: elementwise from the saved maximum, L and H; bound by reading the scores again and writing as much: 8192 x 131072 bf16 755 us,
+// 5.7 TB/s.
 #include "rows_common.h"
 
 namespace {
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * W, E == 64 || (DT == I2P_F32 && E == 32 && W <
 }
 
 // Rows of at most 128 scores: 16 lanes share one (8 scores each, lane by lane), so that a wave has four.  The alternatives are searched one
-// after the other.  60000 x 32 fp32: 21 us with a wave per row, 5.2 here (41 and 12.4 with 3 alternatives)
+// after the other.  60000 x 32 fp32: 20.8 us with a wave per row, 5.5 here (41.7 and 12.7 with 3 alternatives)
 constexpr int SMALL = 128;
 __device__ __forceinline__ skey row16_best(skey k) {
     auto step = [&](unsigned lo, unsigned hi) { const skey u = ((skey)hi << 32) | lo; k = u > k ? u : k; };
@@ -424,9 +425,9 @@ constexpr int FEW = 4096;                       // a slice where blocks are few
 constexpr int SLICE = 8192;                     // 4 waves
 
 // how a row is cut: few rows of up to 32768 scores stay whole, which saves the second launch (the 256 CUs hold two blocks of 16 waves each);
-// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 88 us, slices of 8192 71 + 7; 8192 x 131072: 557,
-// 522 + 13), shorter ones where there would be fewer than half as many as CUs (1 x 131072 fp32: 7.0 -> 6.2 us) and, of the 16-bit types, longer
-// ones where they still fill the chip ten times (8192 x 131072: 492 -> 455 us; 4096 x 32000, which is five times: 72 -> 80)
+// otherwise slices of 4 waves, whose barriers stall less of a CU (4096 x 32000 bf16: whole 73.5 us, slices of 8192 57.5 + 6.1), shorter ones
+// where there would be fewer than half as many as CUs (1 x 131072 fp32: 6.5 -> 5.3 us) and, of the 16-bit types, longer ones where they still
+// fill the chip ten times (8192 x 131072: 508 -> 466 us; 4096 x 32000, which is five times: 58 -> 61)
 inline void cut(long long rows, int v, int dtype, int &nsplit, int &slice) {
     nsplit = v <= WHOLE && rows <= 512 ? 1 : (v + SLICE - 1) / SLICE;
     if (dtype != I2P_F32 && nsplit > 1 && rows * ((nsplit + 1) / 2) >= 16384) nsplit = (v + 2 * SLICE - 1) / (2 * SLICE);
@@ -486,8 +487,8 @@ extern "C" int i2p_token_logprobs_bwd(long long rows, int v, int dtype, const vo
     if (!x || !ids || !stat || !entropy || !dx) return I2P_ERR_BAD_ARG;
     const long long pitch = (long long)v * i2p_esize(dtype);
     // A gradient that no cache would hold until it is used goes past them, and the rows are taken from the last: then what the forward read
-    // last is still in the 256 MB last-level cache (forward + backward 4096 x 32000 bf16: 171 -> 144 us, 8192 x 32000 334 -> 290, with a
-    // consumer of the gradient behind it 264 -> 246 and 502 -> 479).  Rows that do not start on 16 bytes would be written in parts of lines
+    // last is still in the 256 MB last-level cache (kernels of forward + backward in turn, 4096 x 32000 bf16: 163 -> 150 us,
+    // 8192 x 32000 343 -> 326: the forward's 72 and 145 become 58 and 123).  Rows that do not start on 16 bytes would be written in parts of lines
     const bool stream_out = pitch % 16 == 0 && ((uintptr_t)dx & 15) == 0 && rows * pitch >= (64ll << 20);
     by_type(dtype, [&](auto dt) {
         constexpr int DT = dt.value;

@@ -155,7 +155,8 @@ def _norm_kind(norm_type):
 
 def grad_norm(parameters, norm_type=2.0):
     """Global norm (2, or inf: the largest magnitude) of the gradients of `parameters` -> float32 0-d tensor on their device (0 where
-    there is no gradient); the host does not wait.  The norm itself is not differentiable.  `parameters`: parameters, whose .grad is meant (those without one are skipped), or gradient tensors themselves."""
+    there is no gradient); the host does not wait.  The norm itself is not differentiable.  `parameters`: parameters, whose .grad is meant
+    (those without one are skipped), or gradient tensors themselves."""
     return ops.rows().clip_parameters(parameters, _norm_kind(norm_type), None, None)
 
 

@@ -706,7 +706,8 @@ int i2p_kitti_image_build(int B, int out_h, int out_w, const void *table, float 
 /* ---------------------------------------------------------------------------------------------
  * Row operators of a training or matching step (not in the reference): any width, rows of pitch ld >= width (elements), storage types
  * I2P_F32 / I2P_BF16 / I2P_F16, fp32 arithmetic, no alignment beyond the element's own (scratch: 16 bytes).  Results are reproducible.  Sizes outside what is said
- * here, NULL pointers with work and pitches below the width are I2P_ERR_BAD_ARG; no rows is no work.
+ * here, NULL pointers with work and pitches below the width are I2P_ERR_BAD_ARG; no rows is no work (i2p_rms_norm_bwd needs one).  Outputs and
+ * workspaces share no memory with each other or with an input, but for the gradients that i2p_clip_grad_norm scales in place.
  *
  * Root-mean-square norm with the residual's addition: s [rows,d] = round(x + res) (res, s both NULL: the norm is of x itself),
  * d <= I2P_MAX_ROW, rstd f32 [rows] = 1/sqrt(mean(s^2) + eps) (NULL: not wanted), y [rows,d] = round(s * rstd * w); w [d] of type wdtype (I2P_F32 or
