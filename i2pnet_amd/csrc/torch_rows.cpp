@@ -129,8 +129,7 @@ struct Rows {
 variable_list once(variable_list g, const variable_list &from) {
     if (!at::GradMode::is_enabled()) return g;
     torch::autograd::edge_list above = torch::autograd::collect_next_edges(from);
-    const auto inputs = torch::autograd::get_current_node()->next_edges();
-    above.insert(above.end(), inputs.begin(), inputs.end());
+    if (const auto node = torch::autograd::get_current_node()) above.insert(above.end(), node->next_edges().begin(), node->next_edges().end());
     const auto error = std::make_shared<torch::autograd::Error>("trying to differentiate twice a function marked once_differentiable", std::move(above));
     for (auto &t : g)
         if (t.defined()) {
