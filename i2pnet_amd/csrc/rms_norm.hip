@@ -6,7 +6,7 @@
 //   backward, t = gy * w, xh = s * rstd:  dx = dres = round(rstd * (t - xh * mean(t * xh)) + gs),  dw = sum over rows of gy * xh
 //
 // Sums are fp32.  Where the sum of squares passes fp32 (values of 1e19 and more), or would lose digits below it and eps does not cover that
-// (values of 1e-12 and less with an eps as small), it is formed again from scaled values.
+// (values of 1e-12 and less with an eps below 1e-24), it is formed again from scaled values.
 //
 // All of it is bound by memory: a row lives in the registers of the TPR threads that share it (NV 16-byte vectors each, the 16-bit types
 // packed), so every input is read once and every output written once.  Short rows are shared by 16 lanes or one wave (no barrier, several
